@@ -178,6 +178,8 @@ SIGNATURES = {
     "dcd_k_gemm_fma": (I, [P, P, P, I, I, I, I, P]),
     "dcd_k_rmsnorm": (I, [P, P, P, I, I, F, I, I, P]),
     "dcd_k_add_rmsnorm": (I, [P, P, P, P, P, I, I, F, I, P]),
+    "dcd_k_rmsnorm_fp8": (I, [P, SZ, P, P, P, I, I, F, I, F, I, I, P]),
+    "dcd_k_add_rmsnorm_fp8": (I, [P, SZ, P, SZ, P, P, P, P, I, I, F, I, F, I, I, P]),
     "dcd_k_rmsnorm_gated": (I, [P, P, I, P, P, I, I, I, F, I, P]),
     "dcd_k_silu_mul": (I, [P, P, P, SZ, I, P]),
     "dcd_k_add": (I, [P, P, P, SZ, I, P]),
@@ -193,6 +195,12 @@ SIGNATURES = {
     "dcd_k_attention_tc": (I, [P, P, I, P, I, P, P, I, P, I, P, P, P, I, I, I, I, I, P, P]),
     "dcd_k_attention_tc_split": (I, [P, P, I, P, I, P, P, I, P, I, P, P, P, I, I, I, I, I, P, I, P, C.c_size_t, P]),
     "dcd_k_attention_tc_noalloc": (I, [P, P, I, P, I, P, P, I, P, I, P, P, I, I, I, I, I, P, P, C.c_char_p, SZ]),
+    "dcd_k_kv4_write": (I, [P, SZ, P, SZ, P, P, P, P, P, SZ, I, I, I, I, P, P]),
+    "dcd_k_kv4_read": (I, [P, P, P, P, SZ, P, P, P, I, I, I, I, P, P]),
+    "dcd_k_attention_kv4_workspace": (SZ, [I, I, I, I, I, I]),
+    "dcd_k_attention_kv4": (I, [P, SZ, P, SZ, P, SZ, P, P, P, P, I, P, SZ, P, P, I, I, I, I, I, I, P, SZ, P, P]),
+    "dcd_k_attention_kv4_decode_workspace": (SZ, [I, I, I, I, I, I]),
+    "dcd_k_attention_kv4_decode": (I, [P, SZ, P, P, P, P, SZ, P, P, I, P, SZ, P, P, I, I, I, I, I, P, SZ, P, P]),
     "dcd_k_readout": (I, [P, P, P, I, I, I, P]),
 }
 

@@ -15,7 +15,8 @@ enum : int {
   DERR_GEMM_TIMEOUT = 3,  // a bounded mbarrier wait gave up in the tcgen05 GEMM
   DERR_ATTN_TIMEOUT = 4,
   DERR_POSITION_RANGE = 5, // RoPE position beyond the table
-  DERR_GDN_TIMEOUT = 6
+  DERR_GDN_TIMEOUT = 6,
+  DERR_CACHE_ROW = 7      // a row of a 4-bit K/V cache, or a stretch of rows, outside the cache
 };
 
 __device__ __forceinline__ void set_err(int* err, int code) {

@@ -5,6 +5,7 @@
 #include "common.cuh"
 #include "gemm_tcgen05.h"
 #include "kernels.h"
+#include "kv4.h"
 
 namespace {
 inline int rc_of(cudaError_t e) { return e == cudaSuccess ? DCD_OK : (e == cudaErrorInvalidValue ? DCD_E_INVALID : DCD_E_CUDA); }
@@ -138,6 +139,24 @@ int dcd_k_add_rmsnorm(const void* x, const void* mix, const void* w, void* resid
                   launch_add_rmsnorm<bf16>((const bf16*)x, (const bf16*)mix, (const bf16*)w, (bf16*)residual, (bf16*)out, rows, cols, eps, S(stream)));
 }
 
+int dcd_k_rmsnorm_fp8(const void* x, size_t x_stride, const void* w, void* out, float* scales, int rows, int cols, float eps, int zero_centered, float clip,
+                      int round_t, int dtype, void* stream) {
+  if (rows < 0 || cols <= 0 || x_stride < (size_t)cols || !x || !w || !out || !scales) return DCD_E_INVALID;
+  return DISPATCH(dtype,
+                  launch_rmsnorm_fp8<float>((const float*)x, x_stride, nullptr, 0, (const float*)w, nullptr, (uint8_t*)out, scales, rows, cols, eps, zero_centered != 0, clip, round_t != 0, S(stream)),
+                  launch_rmsnorm_fp8<bf16>((const bf16*)x, x_stride, nullptr, 0, (const bf16*)w, nullptr, (uint8_t*)out, scales, rows, cols, eps, zero_centered != 0, clip, round_t != 0, S(stream)));
+}
+
+int dcd_k_add_rmsnorm_fp8(const void* x, size_t x_stride, const void* mix, size_t mix_stride, const void* w, void* residual, void* out, float* scales, int rows,
+                          int cols, float eps, int zero_centered, float clip, int round_t, int dtype, void* stream) {
+  if (rows < 0 || cols <= 0 || x_stride < (size_t)cols || mix_stride < (size_t)cols || !x || !mix || !w || !residual || !out || !scales) return DCD_E_INVALID;
+  // in place only where every element is written where it was read
+  if ((residual == x && x_stride != (size_t)cols) || (residual == mix && mix_stride != (size_t)cols)) return DCD_E_INVALID;
+  return DISPATCH(dtype,
+                  launch_rmsnorm_fp8<float>((const float*)x, x_stride, (const float*)mix, mix_stride, (const float*)w, (float*)residual, (uint8_t*)out, scales, rows, cols, eps, zero_centered != 0, clip, round_t != 0, S(stream)),
+                  launch_rmsnorm_fp8<bf16>((const bf16*)x, x_stride, (const bf16*)mix, mix_stride, (const bf16*)w, (bf16*)residual, (uint8_t*)out, scales, rows, cols, eps, zero_centered != 0, clip, round_t != 0, S(stream)));
+}
+
 int dcd_k_rmsnorm_gated(const void* x, const void* z, int z_stride, const void* w, void* out, int tokens, int heads, int cols, float eps, int dtype, void* stream) {
   return DISPATCH(dtype,
                   launch_rmsnorm_gated<float>((const float*)x, (const float*)z, z_stride, (const float*)w, (float*)out, tokens, heads, cols, eps, S(stream)),
@@ -269,6 +288,75 @@ int dcd_k_attention_tc_split(const void* q, const void* k_own, int k_stride, con
   cudaError_t ce = attn_tc_build_tiles(cu_seqlens, B, tt, tile_cu, S(stream));
   if (ce != cudaSuccess) return rc_of(ce);
   return rc_of(attn_tc_launch(&maps, cu_seqlens, tile_cu, B, n_state, T, max_tiles, heads, kv, hd, gate_qg, qg_stride, out, err, S(stream), n_split, workspace));
+}
+
+namespace {
+// 16-byte steps: pointer aligned, row stride a multiple of 8 bf16 elements
+inline bool rows_ok(const void* p, size_t stride, size_t width) { return p && reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride >= width && stride % 8 == 0; }
+inline bool cache_ok(const void* kc, const void* ks, const void* vc, const void* vs) {
+  return kc && ks && vc && vs && (reinterpret_cast<uintptr_t>(kc) | reinterpret_cast<uintptr_t>(vc) | reinterpret_cast<uintptr_t>(ks) | reinterpret_cast<uintptr_t>(vs)) % 16 == 0;
+}
+inline bool heads_ok(int heads, int kv, int hd) { return kv > 0 && heads > 0 && heads % kv == 0 && heads <= 65535 && kv4_head_dim_ok(hd); }
+inline Kv4Cache cache_of(const void* kc, const void* ks, const void* vc, const void* vs) {
+  return {{(const uint8_t*)kc, (const uint8_t*)ks}, {(const uint8_t*)vc, (const uint8_t*)vs}};
+}
+}  // namespace
+
+int dcd_k_kv4_write(const void* k, size_t k_stride, const void* v, size_t v_stride, const int64_t* slots, void* k_codes, void* k_scales, void* v_codes,
+                    void* v_scales, size_t cache_rows, int rows, int kv, int hd, int dtype, int* err, void* stream) {
+  if (rows < 0 || kv <= 0 || !kv4_head_dim_ok(hd) || k_stride < (size_t)kv * hd || v_stride < (size_t)kv * hd) return DCD_E_INVALID;
+  if (!k || !v || !cache_ok(k_codes, k_scales, v_codes, v_scales) || (!slots && (size_t)rows > cache_rows)) return DCD_E_INVALID;
+  return DISPATCH(dtype,
+                  launch_kv4_write<float>((const float*)k, k_stride, (const float*)v, v_stride, slots, (uint8_t*)k_codes, (uint8_t*)k_scales, (uint8_t*)v_codes, (uint8_t*)v_scales, cache_rows, rows, kv, hd, err, S(stream)),
+                  launch_kv4_write<bf16>((const bf16*)k, k_stride, (const bf16*)v, v_stride, slots, (uint8_t*)k_codes, (uint8_t*)k_scales, (uint8_t*)v_codes, (uint8_t*)v_scales, cache_rows, rows, kv, hd, err, S(stream)));
+}
+
+int dcd_k_kv4_read(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, size_t cache_rows, const int64_t* slots, void* k,
+                   void* v, int rows, int kv, int hd, int dtype, int* err, void* stream) {
+  if (rows < 0 || kv <= 0 || !kv4_head_dim_ok(hd) || !k || !v || (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 != 0) return DCD_E_INVALID;
+  if (!cache_ok(k_codes, k_scales, v_codes, v_scales) || (!slots && (size_t)rows > cache_rows)) return DCD_E_INVALID;
+  const Kv4Cache c = cache_of(k_codes, k_scales, v_codes, v_scales);
+  return DISPATCH(dtype, launch_kv4_read<float>(c, cache_rows, slots, (float*)k, (float*)v, rows, kv, hd, err, S(stream)),
+                  launch_kv4_read<bf16>(c, cache_rows, slots, (bf16*)k, (bf16*)v, rows, kv, hd, err, S(stream)));
+}
+
+size_t dcd_k_attention_kv4_workspace(int B, int T, int n_state, int heads, int kv, int hd) {
+  if (B <= 0 || T <= 0 || n_state < 0 || !heads_ok(heads, kv, hd)) return 0;
+  return kv4_question_workspace(B, T, n_state, heads, kv, hd);
+}
+
+int dcd_k_attention_kv4(const void* q, size_t q_stride, const void* k_own, size_t k_stride, const void* v_own, size_t v_stride, const void* k_codes,
+                        const void* k_scales, const void* v_codes, const void* v_scales, int n_state, const void* gate_qg, size_t qg_stride, void* out,
+                        const int32_t* cu_seqlens, int B, int T, int heads, int kv, int hd, int causal, void* workspace, size_t workspace_bytes, int* err,
+                        void* stream) {
+  if (B <= 0 || T <= 0 || n_state < 0 || !heads_ok(heads, kv, hd)) return DCD_E_INVALID;
+  if (!rows_ok(q, q_stride, (size_t)heads * hd) || !rows_ok(k_own, k_stride, (size_t)kv * hd) || !rows_ok(v_own, v_stride, (size_t)kv * hd)) return DCD_E_INVALID;
+  if ((n_state > 0 && !cache_ok(k_codes, k_scales, v_codes, v_scales)) || (gate_qg && !rows_ok(gate_qg, qg_stride, (size_t)2 * heads * hd))) return DCD_E_INVALID;
+  if (!out || reinterpret_cast<uintptr_t>(out) % 16 != 0 || !cu_seqlens) return DCD_E_INVALID;
+  const size_t need = kv4_question_workspace(B, T, n_state, heads, kv, hd);
+  if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)) return DCD_E_INVALID;
+  Kv4QuestionArgs a{(const bf16*)q, (const bf16*)k_own, (const bf16*)v_own, (const bf16*)gate_qg, q_stride, k_stride, v_stride, qg_stride,
+                    cache_of(k_codes, k_scales, v_codes, v_scales), n_state, (bf16*)out, cu_seqlens, B, T, heads, kv, hd, causal != 0, err};
+  return rc_of(launch_kv4_questions(a, workspace, S(stream)));
+}
+
+size_t dcd_k_attention_kv4_decode_workspace(int B, int T, int max_len, int heads, int kv, int hd) {
+  if (B <= 0 || T <= 0 || max_len < 0 || !heads_ok(heads, kv, hd)) return 0;
+  return kv4_decode_workspace(B, T, max_len, heads, kv, hd);
+}
+
+int dcd_k_attention_kv4_decode(const void* q, size_t q_stride, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+                               size_t cache_rows, const int64_t* seg_start, const int32_t* seg_len, int max_len, const void* gate_qg, size_t qg_stride, void* out,
+                               const int32_t* cu_seqlens, int B, int T, int heads, int kv, int hd, void* workspace, size_t workspace_bytes, int* err,
+                               void* stream) {
+  if (B <= 0 || T <= 0 || max_len < 0 || !heads_ok(heads, kv, hd) || !rows_ok(q, q_stride, (size_t)heads * hd)) return DCD_E_INVALID;
+  if (!cache_ok(k_codes, k_scales, v_codes, v_scales) || !seg_start || !seg_len || (gate_qg && !rows_ok(gate_qg, qg_stride, (size_t)2 * heads * hd))) return DCD_E_INVALID;
+  if (!out || reinterpret_cast<uintptr_t>(out) % 16 != 0 || !cu_seqlens) return DCD_E_INVALID;
+  const size_t need = kv4_decode_workspace(B, T, max_len, heads, kv, hd);
+  if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)) return DCD_E_INVALID;
+  Kv4DecodeArgs a{(const bf16*)q, (const bf16*)gate_qg, q_stride, qg_stride, cache_of(k_codes, k_scales, v_codes, v_scales), cache_rows, seg_start, seg_len,
+                  max_len, (bf16*)out, cu_seqlens, B, T, heads, kv, hd, err};
+  return rc_of(launch_kv4_decode(a, workspace, S(stream)));
 }
 
 int dcd_k_readout(const float* x, const float* W, float* out, int B, int H, int R, void* stream) {

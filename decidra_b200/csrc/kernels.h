@@ -119,6 +119,12 @@ cudaError_t launch_gdn_wy(const TcTensorMap maps[3], const T* conv, int conv_str
 template <typename T>
 cudaError_t launch_quant_fp8_rows(const T* x, size_t x_stride, uint8_t* out, float* scales, int rows, int cols, float clip, cudaStream_t s);
 
+// RMSNorm (mix != nullptr: residual = T(x + mix) first) straight to e4m3 rows and their scales (norm_fp8.cu). round_t: the row is rounded to T
+// before it is quantised, which gives the bits of launch_rmsnorm / launch_add_rmsnorm followed by launch_quant_fp8_rows.
+template <typename T>
+cudaError_t launch_rmsnorm_fp8(const T* x, size_t x_stride, const T* mix, size_t mix_stride, const T* w, T* residual, uint8_t* out, float* scales, int rows,
+                               int cols, float eps, bool zero_centered, float clip, bool round_t, cudaStream_t s);
+
 // W4A16 group-128 weights: packed [N, K/8] words (nibble k of word j = input 8j+k, zero-point 8) and
 // fp16 scales [N, ceil(K/128)]. K % 8 == 0.
 // perm: words in the engine's nibble order [k0 k2 k4 k6 k1 k3 k5 k7] instead of the compressed-tensors order k0..k7

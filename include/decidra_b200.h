@@ -555,6 +555,18 @@ DCD_API int dcd_k_gemm_fma(const void* X, const void* W, void* C, int M, int N, 
 /* rmsnorm_bf16 / add_rmsnorm_bf16 (native/kernels/kernels.cu:378-426). */
 DCD_API int dcd_k_rmsnorm(const void* x, const void* w, void* out, int rows, int cols, float eps, int zero_centered, int dtype, void* stream);
 DCD_API int dcd_k_add_rmsnorm(const void* x, const void* mix, const void* w, void* residual, void* out, int rows, int cols, float eps, int dtype, void* stream);
+/* The same norms writing the operand of dcd_k_gemm_fp8_tc (rmsnorm_bf16 / add_rmsnorm_bf16 followed by quant_fp8_per_token_bf16,
+ * native/kernels/kernels.cu:378-426, 182-205), one launch, the row read once:
+ *   r = x, or T(x + mix), which goes to residual [rows, cols]; y = r / sqrt(mean(r^2) + eps) * (w + zero_centered);
+ *   scales[row] = max(max|y| * clip, 1e-10) / 448; out [rows, cols] = e4m3_satfinite(y / scale).
+ * x and mix are T with row strides in elements; residual may be x or mix itself where that one's stride is cols, and overlaps them in
+ * no other way. round_t != 0 rounds y to T before it is quantised: the bits of dcd_k_rmsnorm / dcd_k_add_rmsnorm (zero_centered 1)
+ * followed by dcd_k_quant_fp8_rows. round_t 0: y stays in f32 and is rounded once. Any cols; fastest where cols and the strides are
+ * multiples of 8 (bf16) or 4 (f32) and the pointers 16-byte aligned. rows 0 does nothing. */
+DCD_API int dcd_k_rmsnorm_fp8(const void* x, size_t x_stride, const void* w, void* out, float* scales, int rows, int cols, float eps, int zero_centered,
+                              float clip, int round_t, int dtype, void* stream);
+DCD_API int dcd_k_add_rmsnorm_fp8(const void* x, size_t x_stride, const void* mix, size_t mix_stride, const void* w, void* residual, void* out,
+                                  float* scales, int rows, int cols, float eps, int zero_centered, float clip, int round_t, int dtype, void* stream);
 /* rmsnorm_gated_bf16 (native/kernels/kernels.cu:430-455): x [tokens*heads, cols], gate z read at
  * z + t*z_stride + head*cols. */
 DCD_API int dcd_k_rmsnorm_gated(const void* x, const void* z, int z_stride, const void* w, void* out, int tokens, int heads, int cols, float eps, int dtype, void* stream);
@@ -654,6 +666,42 @@ DCD_API int dcd_k_attention_tc_noalloc(const void* q, const void* k_own, int k_s
                                        const void* k_state, const void* v_state, int n_state, const void* gate_qg, int qg_stride,
                                        void* out, const int32_t* cu_seqlens, int B, int T, int heads, int kv, int hd, int* err,
                                        void* stream, char* msg, size_t msg_len);
+/* ---- a K/V cache held in 4 bits, and attention over it (no counterpart in the reference, whose caches are bf16: this keeps 3.5 times
+ * the tokens in the same memory) ----
+ * A cache is four arrays: for K and for V, codes [cache_rows, kv, hd / 2] (e2m1, the even dimension in the low nibble) and scales
+ * [cache_rows, kv, hd / 16] (e4m3, one per 16 dimensions), all 16-byte aligned; a value is code * scale. It is the row format of
+ * dcd_k_nvfp4_quant_rows with K = kv * hd and global 1, and the same rule makes the codes: sf = e4m3(max(absmax16 / 6, 1e-10)),
+ * code = e2m1(v / sf), ties up. Magnitudes above 2688 saturate; a NaN is stored as some value of its group. hd: 64, 128 or 256.
+ *
+ * write: token i's K and V (T rows with strides in elements) go to cache row slots[i]; slots == NULL: row i. A negative slot leaves
+ * its token out; a slot >= cache_rows sets *err and is left out. The slots of one call are distinct.
+ * read: cache row slots[i] (or i) to row i of k and v, [rows, kv, hd] T, 16-byte aligned; code * scale is exact in T. Rows of
+ * negative or bad slots are left as they were. rows 0 does nothing; err may be NULL. */
+DCD_API int dcd_k_kv4_write(const void* k, size_t k_stride, const void* v, size_t v_stride, const int64_t* slots, void* k_codes, void* k_scales,
+                            void* v_codes, void* v_scales, size_t cache_rows, int rows, int kv, int hd, int dtype, int* err, void* stream);
+DCD_API int dcd_k_kv4_read(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, size_t cache_rows, const int64_t* slots,
+                           void* k, void* v, int rows, int kv, int hd, int dtype, int* err, void* stream);
+/* dcd_k_attention_tc over a 4-bit state: every packed question attends to the n_state rows of the cache and to its own bf16 keys (all
+ * of them, or with causal != 0 those up to itself), out = softmax(q k / sqrt(hd)) v, times sigmoid(gate) where gate_qg (laid out as
+ * there) is given. n_state 0 with causal 1 is causal attention over packed prompts; the cache pointers may then be NULL. bf16; any
+ * heads that kv divides; hd 64, 128 or 256; q [T, heads, hd], k_own and v_own [T, kv, hd] with row strides in elements, multiples of 8,
+ * 16-byte aligned; out [T, heads, hd]. cu_seqlens [B + 1] rises from 0 to at most T; rows of out behind the last sequence
+ * are left as they were. workspace: dcd_k_attention_kv4_workspace bytes (0: none is needed), 16-byte aligned, not shared by calls that
+ * may overlap. */
+DCD_API size_t dcd_k_attention_kv4_workspace(int B, int T, int n_state, int heads, int kv, int hd);
+DCD_API int dcd_k_attention_kv4(const void* q, size_t q_stride, const void* k_own, size_t k_stride, const void* v_own, size_t v_stride, const void* k_codes,
+                                const void* k_scales, const void* v_codes, const void* v_scales, int n_state, const void* gate_qg, size_t qg_stride,
+                                void* out, const int32_t* cu_seqlens, int B, int T, int heads, int kv, int hd, int causal, void* workspace,
+                                size_t workspace_bytes, int* err, void* stream);
+/* The form for new tokens: sequence b's rows in the cache are [seg_start[b], seg_start[b] + seg_len[b]), its packed tokens
+ * [cu_seqlens[b], cu_seqlens[b + 1]) are the newest ones, already written there: the last token sees every row of the stretch, each
+ * one before it a row less. Stretches may be shared or overlap. A token that sees no row (more tokens than rows) gives 0. A stretch that leaves the cache or is longer
+ * than max_len sets *err, and its tokens give 0. Meant for one to a few tokens a sequence; every other operand as above. */
+DCD_API size_t dcd_k_attention_kv4_decode_workspace(int B, int T, int max_len, int heads, int kv, int hd);
+DCD_API int dcd_k_attention_kv4_decode(const void* q, size_t q_stride, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+                                       size_t cache_rows, const int64_t* seg_start, const int32_t* seg_len, int max_len, const void* gate_qg,
+                                       size_t qg_stride, void* out, const int32_t* cu_seqlens, int B, int T, int heads, int kv, int hd, void* workspace,
+                                       size_t workspace_bytes, int* err, void* stream);
 /* logits[B,R] = x[B,H] . W[R,H]^T in f32 (blas_gemm_f32, native/src/engine.rs:3873-3901, 4977-4984). */
 DCD_API int dcd_k_readout(const float* x, const float* W, float* out, int B, int H, int R, void* stream);
 
