@@ -93,35 +93,6 @@ __global__ void __launch_bounds__(32) kv4_questions_kernel(const Kv4QuestionArgs
   store_row<D>(r, a.out + ((size_t)t * a.heads + h) * HD, a.gate_qg ? a.gate_qg + t * a.qg_stride + (size_t)h * 2 * HD + HD : nullptr, lane);
 }
 
-template <int D>
-__global__ void __launch_bounds__(32) kv4_decode_kernel(const Kv4DecodeArgs a) {
-  constexpr int HD = 32 * D;
-  const int t = blockIdx.x, h = blockIdx.y, kh = h / (a.heads / a.kv), lane = threadIdx.x;
-  const int b = sequence_of(a.cu, a.B, t);
-  if (b < 0) return;
-  const float scale = 1.0f / sqrtf((float)HD);
-  int64_t start = a.seg_start[b];
-  int len = a.seg_len[b];
-  if (start < 0 || len < 0 || len > a.max_len || (uint64_t)start > a.cache_rows || (uint64_t)len > a.cache_rows - (uint64_t)start) {
-    set_err(a.err, DERR_CACHE_ROW);
-    len = 0;
-  }
-  const int end = len - (a.cu[b + 1] - 1 - t);  // the last token of the sequence sees all rows
-  float q[D], k[D], v[D];
-  Running<D> r;
-#pragma unroll
-  for (int i = 0; i < D; ++i) {
-    q[i] = __bfloat162float(a.q[t * a.q_stride + (size_t)h * HD + lane * D + i]);
-    r.o[i] = 0.f;
-  }
-  for (int j = 0; j < end; ++j) {
-    cache_values<D>(a.cache.k, (size_t)start + j, a.kv, kh, lane, k);
-    cache_values<D>(a.cache.v, (size_t)start + j, a.kv, kh, lane, v);
-    r.add(q, k, v, scale);
-  }
-  store_row<D>(r, a.out + ((size_t)t * a.heads + h) * HD, a.gate_qg ? a.gate_qg + t * a.qg_stride + (size_t)h * 2 * HD + HD : nullptr, lane);
-}
-
 }  // namespace
 
 size_t kv4_question_workspace(int, int, int, int, int, int) { return 0; }
@@ -130,14 +101,5 @@ cudaError_t launch_kv4_questions(const Kv4QuestionArgs& a, void*, cudaStream_t s
   if (a.hd == 64) kv4_questions_kernel<2><<<grid, 32, 0, s>>>(a);
   else if (a.hd == 128) kv4_questions_kernel<4><<<grid, 32, 0, s>>>(a);
   else kv4_questions_kernel<8><<<grid, 32, 0, s>>>(a);
-  return cudaGetLastError();
-}
-
-size_t kv4_decode_workspace(int, int, int, int, int, int) { return 0; }
-cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, void*, cudaStream_t s) {
-  const dim3 grid(a.T, a.heads);
-  if (a.hd == 64) kv4_decode_kernel<2><<<grid, 32, 0, s>>>(a);
-  else if (a.hd == 128) kv4_decode_kernel<4><<<grid, 32, 0, s>>>(a);
-  else kv4_decode_kernel<8><<<grid, 32, 0, s>>>(a);
   return cudaGetLastError();
 }

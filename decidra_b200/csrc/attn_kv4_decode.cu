@@ -1,0 +1,554 @@
+// Attention of the newest tokens of many sequences over their stretches of a 4-bit K/V cache (dcd_k_attention_kv4_decode).
+//
+// One CTA = (sequence, K/V head, chunk of its keys); its four warps take the chunk's blocks of 32 keys in turn, each with a ring of
+// blocks of its own in shared memory (cp.async, no barrier between warps). Few query rows share each key (tokens x heads of the
+// group, eight per MMA column tile), so the kernel lives on getting 0.5625 bytes a value from HBM into matrix fragments:
+//   S^T[16 keys, 8 rows]  += K[16 keys, 16 dims] Q^T      mma.m16n8k16 with the KEYS as the 16-row operand: all of it is used
+//   O^T[16 dims, 8 rows]  += V^T[16 dims, 16 keys] P^T    even for one token of six heads, where rows as M would fill 6 of 16
+// The fragments are made in registers straight from the code words. The order of the contracted dimensions is free as long as Q has
+// the same, so a lane's K values are 16 (head_dim 64) to 64 (256) consecutive dimensions of two keys, loaded 16 bytes at a time; a
+// lane's V values are 8 to 32 consecutive dimensions of four keys, and the code words of two neighbouring keys are merged nibble by
+// nibble first, so that one conversion instruction (cvt.rn.f16x2.e2m1x2, which picks its byte for free: 182 values per ns and SM
+// measured with the scale's product, against 63 for shifting bits into place and 79 needed at HBM speed) gives the pair (key, key + 1)
+// of one dimension that the fragment wants. code * scale is exact in f16. P^T comes from S^T with one 8 x 8 transpose per 16 keys.
+//
+// Q is bf16 and the products f16: each row is divided by the power of two of its largest value (exact but for elements below 2^-14 of
+// it, which keep an absolute error of 2^-25 of it), and the factor returns in the softmax scale. P is held as p * 2^10 in f16, so
+// that weights down to 2^-34 of the row's largest survive. Maxima, sums and O are f32.
+//
+// Long stretches are cut into chunks (kv4_decode_chunk); each leaves its unnormalised O with maximum and sum in the workspace, and a
+// second kernel adds them up. Keys beyond the stretch are zero-filled, masked keys get p = 0.
+#include "common.cuh"
+#include "kv4.h"
+
+namespace kvd {
+
+constexpr int WARPS = 4, KB = 32, STAGES = 3;
+constexpr float P_SHIFT = 10.0f;  // P is held as p * 2^10
+
+template <int HD> struct Ring {
+  static constexpr int ROW = HD / 2, SROW = HD / 16;                            // bytes of a key's codes and scales
+  static constexpr int K = 0, V = KB * ROW, KS = 2 * KB * ROW, VS = KS + KB * SROW;
+  static constexpr int BYTES = VS + KB * SROW;
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+template <int N>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool valid) {  // zeros where !valid
+  const int n = valid ? N : 0;
+  if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// the four byte pairs of codes in w as f16x2 (low nibble in the low half)
+__device__ __forceinline__ void e2m1x8(uint32_t w, uint32_t (&v)[4]) {
+  asm("{\n.reg .b8 b0, b1, b2, b3;\nmov.b32 {b0, b1, b2, b3}, %4;\n"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\ncvt.rn.f16x2.e2m1x2 %1, b1;\ncvt.rn.f16x2.e2m1x2 %2, b2;\ncvt.rn.f16x2.e2m1x2 %3, b3;\n}"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+      : "r"(w));
+}
+__device__ __forceinline__ uint32_t e4m3x2(uint32_t two) {  // two scales (low 16 bits) as f16x2
+  uint32_t r;
+  asm("{\n.reg .b16 h, t;\nmov.b32 {h, t}, %1;\ncvt.rn.f16x2.e4m3x2 %0, h;\n}" : "=r"(r) : "r"(two));
+  return r;
+}
+__device__ __forceinline__ uint32_t hmul(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) { return __byte_perm(a, b, s); }
+
+// Shared-memory position of 16-byte chunk `c` of key `k`: a quarter-warp reads two keys' four chunks (K) or four keys' two (V), which
+// for rows of 128 bytes would meet in the same banks.
+template <int HD> __device__ __forceinline__ int k_chunk(int k, int c) { return HD == 256 ? c ^ ((k & 1) << 2) : c; }
+template <int HD> __device__ __forceinline__ int v_chunk(int k, int c) { return HD == 256 ? c ^ (k & 6) : HD == 128 ? c ^ (k & 2) : c; }
+
+struct Args {
+  Kv4DecodeArgs a;
+  int chunk;       // keys per chunk
+  int n_chunks;    // chunks of max_len; with more than one, the parts go to the workspace
+  float* ws_o;     // [T * heads][n_chunks][hd]
+  float2* ws_ml;   // [T * heads][n_chunks] (maximum in log2 units, sum)
+};
+
+struct Sequence {
+  int off, L, len;
+  size_t start;
+};
+// Bounds-checked view of sequence b; a bad one has no tokens or no rows.
+__device__ __forceinline__ Sequence sequence(const Kv4DecodeArgs& a, int b, bool report) {
+  Sequence s;
+  s.off = a.cu[b];
+  s.L = a.cu[b + 1] - s.off;
+  if (s.off < 0 || s.L < 0 || s.L > a.T - s.off) {
+    if (report) set_err(a.err, DERR_OFFSETS);
+    s.L = 0;
+  }
+  const int64_t st = a.seg_start[b];
+  s.len = a.seg_len[b];
+  s.start = (size_t)st;
+  if (st < 0 || s.len < 0 || s.len > a.max_len || (uint64_t)st > a.cache_rows || (uint64_t)s.len > a.cache_rows - (uint64_t)st) {
+    if (report) set_err(a.err, DERR_CACHE_ROW);
+    s.len = 0;
+    s.start = 0;
+  }
+  return s;
+}
+
+// out row of head_dim values: normalised, gated, rounded once. n consecutive values of one thread.
+__device__ __forceinline__ float gated(float o, const bf16* gate, int d) {
+  return gate ? o * sigmoid_f(__bfloat162float(gate[d])) : o;
+}
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(WARPS * 32, 2) kv4_decode_kernel(const Args p) {
+  using R = Ring<HD>;
+  constexpr int KW = HD / 32;               // K code words of a lane per key
+  constexpr int KL = KW < 4 ? KW : 4;       // ... loaded at once
+  constexpr int VW = HD / 64;               // V code words of a lane per key
+  constexpr int ROWS = 8 * NT;
+  constexpr bool Q_SMEM = NT * HD > 256;    // Q fragments from shared memory where registers run out
+  const Kv4DecodeArgs& a = p.a;
+  const int b = blockIdx.z, kh = blockIdx.y, z = blockIdx.x;
+  const Sequence sq = sequence(a, b, z == 0 && kh == 0 && threadIdx.x == 0);
+  const int k0 = z * p.chunk, k1 = min(sq.len, k0 + p.chunk);  // this chunk's keys, relative to the stretch
+  if (p.n_chunks > 1 && k0 >= k1) return;                      // the merge reads only chunks that hold keys
+  const int G = a.heads / a.kv, n_rows = sq.L * G;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint8_t* ring = smem + warp * (STAGES * R::BYTES);
+  const uint32_t ring_addr = smem_addr(ring);
+  uint2* q_smem = reinterpret_cast<uint2*>(smem + WARPS * STAGES * R::BYTES);  // [word * 2 + half][nt][lane]
+  const float scale_log2e = (1.0f / sqrtf((float)HD)) * 1.4426950408889634f;
+  const int n_blocks = k1 > k0 ? (k1 - k0 + KB - 1) / KB : 0;
+
+  // rows of the cache for this head
+  const size_t row0 = (sq.start + (size_t)k0) * a.kv + kh;
+  const uint8_t* kc = a.cache.k.codes + row0 * R::ROW;
+  const uint8_t* vc = a.cache.v.codes + row0 * R::ROW;
+  const uint8_t* ks = a.cache.k.scales + row0 * R::SROW;
+  const uint8_t* vs = a.cache.v.scales + row0 * R::SROW;
+  const size_t code_step = (size_t)a.kv * R::ROW, scale_step = (size_t)a.kv * R::SROW;
+
+  auto fetch = [&](int blk, int slot) {
+    const int j0 = blk * KB, left = (k1 - k0) - j0;  // keys of the block that exist
+    const uint32_t base = ring_addr + slot * R::BYTES;
+    constexpr int CH = R::ROW / 16;
+#pragma unroll
+    for (int i = 0; i < KB * CH / 32; ++i) {
+      const int id = lane + 32 * i, key = id / CH, ch = id % CH;
+      const bool ok = key < left;
+      const size_t at = (size_t)(ok ? j0 + key : 0) * code_step + ch * 16;
+      cp_async<16>(base + R::K + key * R::ROW + k_chunk<HD>(key, ch) * 16, kc + at, ok);
+      cp_async<16>(base + R::V + key * R::ROW + v_chunk<HD>(key, ch) * 16, vc + at, ok);
+    }
+    const bool ok = lane < left;  // one key's scales per lane
+    const size_t at = (size_t)(ok ? j0 + lane : 0) * scale_step;
+    cp_async<R::SROW>(base + R::KS + lane * R::SROW, ks + at, ok);
+    cp_async<R::SROW>(base + R::VS + lane * R::SROW, vs + at, ok);
+  };
+
+  for (int r0 = 0; r0 < n_rows; r0 += ROWS) {  // one round but for many tokens
+    // ---- the first blocks are on their way before Q is read -----------------------------------------
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) {
+      if (warp + i * WARPS < n_blocks) fetch(warp + i * WARPS, i);
+      cp_commit();
+    }
+    // ---- Q as the column operand: lane (g, c) holds row g's dimensions of quad position c -------------
+    uint2 qf[Q_SMEM ? 1 : NT][Q_SMEM ? 1 : KW * 2];
+    float f[NT][2];  // softmax factor of rows 2c, 2c + 1
+    int end[NT][2];  // first key (relative to the chunk) that the row does not see
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = r0 + nt * 8 + g;
+      const bool live = row < n_rows;
+      const bf16* src = live ? a.q + (size_t)(sq.off + row / G) * a.q_stride + (size_t)(kh * G + row % G) * HD : a.q;
+      uint4 u[KW];
+      float m = 0.f;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        const int d = HD == 256 ? (w >> 2) * 128 + 32 * c + 8 * (w & 3) : KL * 8 * c + 8 * w;
+        u[w] = live ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u[w]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(fabsf(__low2float(h[i])), fabsf(__high2float(h[i]))));
+      }
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      // 2^e <= m < 2^(e+1); a row of zeros and one of infinities keep their values
+      const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -126), 126);
+      const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u[w]);
+        uint32_t v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = pack_f16(__low2float(h[i]) * inv, __high2float(h[i]) * inv);
+        if constexpr (Q_SMEM) {
+          if (warp == 0) {
+            q_smem[((2 * w) * NT + nt) * 32 + lane] = make_uint2(v[0], v[1]);
+            q_smem[((2 * w + 1) * NT + nt) * 32 + lane] = make_uint2(v[2], v[3]);
+          }
+        } else {
+          qf[nt][2 * w] = make_uint2(v[0], v[1]);
+          qf[nt][2 * w + 1] = make_uint2(v[2], v[3]);
+        }
+      }
+      const float fr = scale_log2e * __uint_as_float((uint32_t)(127 + e) << 23);
+      f[nt][0] = __shfl_sync(0xffffffffu, fr, 8 * c);
+      f[nt][1] = __shfl_sync(0xffffffffu, fr, 8 * c + 4);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int rr = min(r0 + nt * 8 + 2 * c + i, n_rows - 1);
+        end[nt][i] = min(sq.len - (sq.L - 1 - rr / G), k1) - k0;
+      }
+    }
+    if constexpr (Q_SMEM) __syncthreads();
+
+    float o[HD / 16][NT][4];
+#pragma unroll
+    for (int t = 0; t < HD / 16; ++t)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[t][nt][i] = 0.f;
+    float m[NT][2], l[NT][2];
+    int first_end = end[0][0];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        m[nt][i] = -INFINITY;
+        l[nt][i] = 0.f;
+        first_end = min(first_end, end[nt][i]);
+      }
+
+    int slot = 0;
+    for (int blk = warp; blk < n_blocks; blk += WARPS) {
+      if (blk + (STAGES - 1) * WARPS < n_blocks) fetch(blk + (STAGES - 1) * WARPS, slot == 0 ? STAGES - 1 : slot - 1);
+      cp_commit();
+      cp_wait<STAGES - 1>();
+      __syncwarp();
+      const uint8_t* st = ring + slot * R::BYTES;
+
+      // ---- S^T of two 16-key tiles ------------------------------------------------------------------
+      float s[2][NT][4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[t][nt][i] = 0.f;
+#pragma unroll
+      for (int ld = 0; ld < KW / KL; ++ld) {
+        uint32_t w[4][KL];   // [tile * 2 + (key + 8)][word]
+        uint32_t sc[4];      // the keys' scales of this load, f16x2
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = (i >> 1) * 16 + (i & 1) * 8 + g;
+          if constexpr (KL == 4) {
+            const uint4 u = *reinterpret_cast<const uint4*>(st + R::K + key * R::ROW + k_chunk<HD>(key, ld * 4 + c) * 16);
+            w[i][0] = u.x; w[i][1] = u.y; w[i][2] = u.z; w[i][3] = u.w;
+            sc[i] = e4m3x2(*reinterpret_cast<const uint16_t*>(st + R::KS + key * R::SROW + ld * 8 + 2 * c));
+          } else {
+            const uint2 u = *reinterpret_cast<const uint2*>(st + R::K + key * R::ROW + c * 8);
+            w[i][0] = u.x; w[i][1] = u.y;
+            sc[i] = e4m3x2((uint32_t)st[R::KS + key * R::SROW + c]);
+          }
+        }
+#pragma unroll
+        for (int wi = 0; wi < KL; ++wi) {
+          uint32_t av[4][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t s2 = prmt(sc[i], 0, wi < 2 ? 0x1010 : 0x3232);  // two words share a scale
+            e2m1x8(w[i][wi], av[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) av[i][j] = hmul(av[i][j], s2);
+          }
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const int step = (ld * KL + wi) * 2 + half;
+              const uint2 q = Q_SMEM ? q_smem[(step * NT + nt) * 32 + lane] : qf[Q_SMEM ? 0 : nt][Q_SMEM ? 0 : step];
+#pragma unroll
+              for (int t = 0; t < 2; ++t) mma(s[t][nt], av[2 * t][2 * half], av[2 * t + 1][2 * half], av[2 * t][2 * half + 1], av[2 * t + 1][2 * half + 1], q.x, q.y);
+            }
+        }
+      }
+
+      // ---- softmax: lane (g, c) has keys g, g + 8 of either tile for rows 2c, 2c + 1 --------------------
+      const int j0 = blk * KB;
+      const bool partial = j0 + KB > first_end;
+      uint32_t pb[2][NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float x = s[t][nt][i] * f[nt][i & 1];
+            if (partial && j0 + t * 16 + (i >> 1) * 8 + g >= end[nt][i & 1]) x = -INFINITY;
+            s[t][nt][i] = x;
+            mx[i & 1] = fmaxf(mx[i & 1], x);
+          }
+        float corr[2], neg[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 4));
+          mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 8));
+          mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 16));
+          mx[i] = fmaxf(mx[i], m[nt][i]);
+          const float base = mx[i] == -INFINITY ? 0.f : mx[i];  // a row that has seen nothing yet
+          corr[i] = ex2(m[nt][i] - base);
+          neg[i] = P_SHIFT - base;
+          l[nt][i] *= corr[i];
+        }
+        if (__any_sync(0xffffffffu, mx[0] != m[nt][0] || mx[1] != m[nt][1])) {
+#pragma unroll
+          for (int t = 0; t < HD / 16; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[t][nt][i] *= corr[i & 1];
+        }
+        m[nt][0] = mx[0];
+        m[nt][1] = mx[1];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          float e[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            e[i] = ex2(s[t][nt][i] + neg[i & 1]);
+            l[nt][i & 1] += e[i];
+          }
+          pb[t][nt][0] = transpose8(pack_f16(e[0], e[1]));
+          pb[t][nt][1] = transpose8(pack_f16(e[2], e[3]));
+        }
+      }
+
+      // ---- O^T += V^T P^T: lane (g, c) holds 8 to 32 dimensions of keys 2c, 2c + 1, 2c + 8, 2c + 9 ---------
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        uint32_t w[4][VW], sc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = t * 16 + 2 * c + (i & 1) + (i >> 1) * 8;
+          if constexpr (HD == 256) {
+            const uint4 u = *reinterpret_cast<const uint4*>(st + R::V + key * R::ROW + v_chunk<HD>(key, g) * 16);
+            w[i][0] = u.x; w[i][1] = u.y; w[i][2] = u.z; w[i][3] = u.w;
+            sc[i] = *reinterpret_cast<const uint16_t*>(st + R::VS + key * R::SROW + 2 * g);
+          } else if constexpr (HD == 128) {
+            const uint2 u = *reinterpret_cast<const uint2*>(st + R::V + key * R::ROW + v_chunk<HD>(key, g >> 1) * 16 + (g & 1) * 8);
+            w[i][0] = u.x; w[i][1] = u.y;
+            sc[i] = st[R::VS + key * R::SROW + g];
+          } else {
+            w[i][0] = *reinterpret_cast<const uint32_t*>(st + R::V + key * R::ROW + g * 4);
+            sc[i] = st[R::VS + key * R::SROW + (g >> 1)];
+          }
+        }
+        uint32_t s01[2], s89[2];  // per scale group of the lane: (key, key + 1)
+        if constexpr (HD == 256) {
+          const uint32_t x0 = e4m3x2(sc[0]), x1 = e4m3x2(sc[1]), x2 = e4m3x2(sc[2]), x3 = e4m3x2(sc[3]);
+          s01[0] = prmt(x0, x1, 0x5410); s01[1] = prmt(x0, x1, 0x7632);
+          s89[0] = prmt(x2, x3, 0x5410); s89[1] = prmt(x2, x3, 0x7632);
+        } else {
+          s01[0] = s01[1] = e4m3x2(sc[0] | sc[1] << 8);
+          s89[0] = s89[1] = e4m3x2(sc[2] | sc[3] << 8);
+        }
+#pragma unroll
+        for (int wi = 0; wi < VW; ++wi) {
+          // the two keys' codes of one dimension side by side in a byte: even dimensions, odd dimensions
+          constexpr uint32_t LO = 0x0F0F0F0Fu, HI = 0xF0F0F0F0u;
+          uint32_t ev[4], ov[4], ev8[4], ov8[4];
+          e2m1x8((w[0][wi] & LO) | ((w[1][wi] << 4) & HI), ev);
+          e2m1x8(((w[0][wi] >> 4) & LO) | (w[1][wi] & HI), ov);
+          e2m1x8((w[2][wi] & LO) | ((w[3][wi] << 4) & HI), ev8);
+          e2m1x8(((w[2][wi] >> 4) & LO) | (w[3][wi] & HI), ov8);
+          const uint32_t sa = s01[HD == 256 ? wi >> 1 : 0], sb = s89[HD == 256 ? wi >> 1 : 0];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t a0 = hmul(ev[j], sa), a1 = hmul(ov[j], sa), a2 = hmul(ev8[j], sb), a3 = hmul(ov8[j], sb);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma(o[wi * 4 + j][nt], a0, a1, a2, a3, pb[t][nt][0], pb[t][nt][1]);
+          }
+        }
+      }
+      __syncwarp();  // the slot may be refilled
+      slot = slot + 1 == STAGES ? 0 : slot + 1;
+    }
+    cp_wait<0>();
+    __syncthreads();  // the rings are free: they take the warps' parts
+
+    // ---- the four warps' parts of each row ---------------------------------------------------------------
+    float* part_o = reinterpret_cast<float*>(smem);                       // [warp][row][HD]
+    float2* part_ml = reinterpret_cast<float2*>(smem + WARPS * ROWS * HD * 4);  // [warp][row]
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], 4);
+        l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], 8);
+        l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], 16);
+        const int row = nt * 8 + 2 * c + i;
+        if (g == 0) part_ml[warp * ROWS + row] = make_float2(m[nt][i], l[nt][i]);
+        float* dst = part_o + (size_t)(warp * ROWS + row) * HD + g * (HD / 8);
+#pragma unroll
+        for (int t = 0; t < HD / 16; ++t) *reinterpret_cast<float2*>(dst + 2 * t) = make_float2(o[t][nt][i], o[t][nt][i + 2]);
+      }
+    __syncthreads();
+    const int rows_here = min(ROWS, n_rows - r0);
+    constexpr int PER = HD / 32;  // values of a lane; one warp per row
+    for (int row = warp; row < rows_here; row += WARPS) {
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, part_ml[w * ROWS + row].x);
+      float acc[PER], sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float2 ml = part_ml[w * ROWS + row];
+        const float fw = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+        sum += fw * ml.y;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) acc[i] += fw * part_o[(size_t)(w * ROWS + row) * HD + lane + 32 * i];
+      }
+      const int r = r0 + row, t = sq.off + r / G, h = kh * G + r % G;
+      const size_t at = (size_t)t * a.heads + h;
+      if (p.n_chunks > 1) {
+        if (lane == 0) p.ws_ml[at * p.n_chunks + z] = make_float2(M, sum);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) p.ws_o[(at * p.n_chunks + z) * HD + lane + 32 * i] = acc[i];
+      } else {
+        const bf16* gate = a.gate_qg ? a.gate_qg + (size_t)t * a.qg_stride + (size_t)h * 2 * HD + HD : nullptr;
+        const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) a.out[at * HD + lane + 32 * i] = __float2bfloat16_rn(gated(acc[i] * inv, gate, lane + 32 * i));
+      }
+    }
+    if (r0 + ROWS < n_rows) __syncthreads();  // before the rings are filled again
+  }
+}
+
+// out = sum_z O_z 2^(m_z - M) / sum_z l_z 2^(m_z - M): one warp per (token, head), the parts in their order
+template <int HD>
+__global__ void __launch_bounds__(128) kv4_decode_merge_kernel(const Args p) {
+  constexpr int PER = HD / 32;
+  const Kv4DecodeArgs& a = p.a;
+  const size_t at = (size_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, t = (int)(at / (unsigned)a.heads), h = (int)(at - (size_t)t * a.heads);
+  if (t >= a.T || t >= a.cu[a.B]) return;
+  int lo = 0, hi = a.B;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.cu[mid] <= t) lo = mid; else hi = mid;
+  }
+  const Sequence sq = sequence(a, lo, false);
+  if (sq.L == 0) return;
+  const int nz = (sq.len + p.chunk - 1) / p.chunk;
+  const float2* ml = p.ws_ml + at * p.n_chunks;
+  float M = -INFINITY;
+  for (int z = lane; z < nz; z += 32) M = fmaxf(M, ml[z].x);
+  M = warp_max(M);
+  float acc[PER], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+  if (M != -INFINITY) {
+    const float* src = p.ws_o + at * p.n_chunks * HD + lane * PER;
+#pragma unroll 4
+    for (int z = 0; z < nz; ++z) {
+      const float2 x = ml[z];
+      const float w = ex2(x.x - M);  // a part that saw nothing has m = -inf: weight 0 on zeros
+      sum += w * x.y;
+#pragma unroll
+      for (int i = 0; i < PER; i += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(src + (size_t)z * HD + i);
+        acc[i] += w * v.x;
+        acc[i + 1] += w * v.y;
+      }
+    }
+  }
+  const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+  const bf16* gate = a.gate_qg ? a.gate_qg + (size_t)t * a.qg_stride + (size_t)h * 2 * HD + HD : nullptr;
+#pragma unroll
+  for (int i = 0; i < PER; i += 2) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(gated(acc[i] * inv, gate, lane * PER + i), gated(acc[i + 1] * inv, gate, lane * PER + i + 1));
+    *reinterpret_cast<__nv_bfloat162*>(a.out + at * HD + lane * PER + i) = v;
+  }
+}
+
+int sm_count() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) return 148;
+  return sms;
+}
+
+// Keys per chunk: as long as there are eight CTAs per SM (two resident ones four times over, for the ragged tail), at most 2048 (a
+// part's O is then under 1 % of what its keys weigh) and at least 128 (a block per warp).
+int chunk_of(int B, int kv, int max_len) {
+  int chunk = 2048;
+  while (chunk > 128 && (size_t)B * kv * (((size_t)max_len + chunk - 1) / chunk) < (size_t)8 * sm_count()) chunk >>= 1;
+  return chunk;
+}
+
+template <int HD, int NT>
+cudaError_t run(const Args& p, cudaStream_t s) {
+  constexpr int rings = WARPS * STAGES * Ring<HD>::BYTES, parts = WARPS * 8 * NT * (HD * 4 + 8);
+  constexpr int bytes = (rings + (NT * HD > 256 ? HD / 32 * 2 * NT * 256 : 0)) > parts ? (rings + (NT * HD > 256 ? HD / 32 * 2 * NT * 256 : 0)) : parts;
+  CUDA_TRY(cudaFuncSetAttribute(kv4_decode_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  kv4_decode_kernel<HD, NT><<<dim3(p.n_chunks, p.a.kv, p.a.B), WARPS * 32, bytes, s>>>(p);
+  CUDA_TRY(cudaGetLastError());
+  if (p.n_chunks > 1) {
+    const size_t rows = (size_t)p.a.T * p.a.heads;
+    kv4_decode_merge_kernel<HD><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace kvd
+
+size_t kv4_decode_workspace(int B, int T, int max_len, int heads, int kv, int hd) {
+  const int chunk = kvd::chunk_of(B, kv, max_len);
+  const size_t n = ((size_t)max_len + chunk - 1) / chunk;
+  return n > 1 ? (size_t)T * heads * n * ((size_t)hd * sizeof(float) + sizeof(float2)) : 0;
+}
+
+cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, void* workspace, cudaStream_t s) {
+  if (a.B > 65535 || a.kv > 65535) return cudaErrorInvalidValue;
+  kvd::Args p;
+  p.a = a;
+  p.chunk = kvd::chunk_of(a.B, a.kv, a.max_len);
+  p.n_chunks = a.max_len > p.chunk ? (int)(((size_t)a.max_len + p.chunk - 1) / p.chunk) : 1;
+  p.ws_o = (float*)workspace;
+  p.ws_ml = (float2*)((char*)workspace + (size_t)a.T * a.heads * p.n_chunks * a.hd * sizeof(float));
+  // column tiles of eight rows by the rows of a sequence of average length; longer ones take several rounds over their keys
+  const int rows = ((a.T + a.B - 1) / a.B) * (a.heads / a.kv);
+  if (a.hd == 256) return rows <= 8 ? kvd::run<256, 1>(p, s) : kvd::run<256, 2>(p, s);
+  if (a.hd == 128) return rows <= 8 ? kvd::run<128, 1>(p, s) : rows <= 16 ? kvd::run<128, 2>(p, s) : kvd::run<128, 4>(p, s);
+  return rows <= 8 ? kvd::run<64, 1>(p, s) : rows <= 16 ? kvd::run<64, 2>(p, s) : kvd::run<64, 4>(p, s);
+}

@@ -812,6 +812,7 @@ int check_device_error(dcd_engine* e) {
     case DERR_GEMM_TIMEOUT: return fail(e, DCD_E_TIMEOUT, "tcgen05 GEMM: a bounded barrier wait gave up");
     case DERR_ATTN_TIMEOUT: return fail(e, DCD_E_TIMEOUT, "tcgen05 attention: a bounded barrier wait gave up");
     case DERR_GDN_TIMEOUT: return fail(e, DCD_E_TIMEOUT, "tcgen05 gated delta rule: a bounded barrier wait gave up");
+    case DERR_OFFSETS: return fail(e, DCD_E_INVALID, "packed offsets outside the batch");
     case DERR_CACHE_ROW: return fail(e, DCD_E_INVALID, "row outside the 4-bit K/V cache");
     default: return fail(e, DCD_E_CUDA, "device error word %d", code);
   }

@@ -341,7 +341,7 @@ int dcd_k_attention_kv4(const void* q, size_t q_stride, const void* k_own, size_
 }
 
 size_t dcd_k_attention_kv4_decode_workspace(int B, int T, int max_len, int heads, int kv, int hd) {
-  if (B <= 0 || T <= 0 || max_len < 0 || !heads_ok(heads, kv, hd)) return 0;
+  if (B <= 0 || T <= 0 || max_len < 0 || max_len > (1 << 30) || !heads_ok(heads, kv, hd)) return 0;
   return kv4_decode_workspace(B, T, max_len, heads, kv, hd);
 }
 
@@ -349,7 +349,7 @@ int dcd_k_attention_kv4_decode(const void* q, size_t q_stride, const void* k_cod
                                size_t cache_rows, const int64_t* seg_start, const int32_t* seg_len, int max_len, const void* gate_qg, size_t qg_stride, void* out,
                                const int32_t* cu_seqlens, int B, int T, int heads, int kv, int hd, void* workspace, size_t workspace_bytes, int* err,
                                void* stream) {
-  if (B <= 0 || T <= 0 || max_len < 0 || !heads_ok(heads, kv, hd) || !rows_ok(q, q_stride, (size_t)heads * hd)) return DCD_E_INVALID;
+  if (B <= 0 || T <= 0 || max_len < 0 || max_len > (1 << 30) || !heads_ok(heads, kv, hd) || !rows_ok(q, q_stride, (size_t)heads * hd)) return DCD_E_INVALID;
   if (!cache_ok(k_codes, k_scales, v_codes, v_scales) || !seg_start || !seg_len || (gate_qg && !rows_ok(gate_qg, qg_stride, (size_t)2 * heads * hd))) return DCD_E_INVALID;
   if (!out || reinterpret_cast<uintptr_t>(out) % 16 != 0 || !cu_seqlens) return DCD_E_INVALID;
   const size_t need = kv4_decode_workspace(B, T, max_len, heads, kv, hd);
