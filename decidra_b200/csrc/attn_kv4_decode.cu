@@ -1,8 +1,12 @@
 // Attention of the newest tokens of many sequences over their stretches of a 4-bit K/V cache (dcd_k_attention_kv4_decode).
 //
-// One CTA = (sequence, K/V head, chunk of its keys); its four warps take the chunk's blocks of 32 keys in turn, each with a ring of
-// blocks of its own in shared memory (cp.async, no barrier between warps). Few query rows share each key (tokens x heads of the
-// group, eight per MMA column tile), so the kernel lives on getting 0.5625 bytes a value from HBM into matrix fragments:
+// A pair is a sequence with one K/V head (and, for more query rows than a CTA holds, one round of them); its keys come in blocks of
+// 32. All blocks of all pairs lie behind each other and every CTA of one resident wave takes the same number of them, so sequences of
+// very different lengths keep every SM busy to the end, and a CTA pays its start (offsets, Q, the first loads: about 8 us, as much as
+// 150 keys' streaming per warp) once or twice instead of once per chunk. A CTA's warps take its blocks in
+// turn, each with a ring of blocks of its own in shared memory (cp.async, no barrier between warps). Few query rows share each key
+// (tokens x heads of the group, eight per MMA column tile), so the kernel lives on getting 0.5625 bytes a value from HBM into
+// matrix fragments:
 //   S^T[16 keys, 8 rows]  += K[16 keys, 16 dims] Q^T      mma.m16n8k16 with the KEYS as the 16-row operand: all of it is used
 //   O^T[16 dims, 8 rows]  += V^T[16 dims, 16 keys] P^T    even for one token of six heads, where rows as M would fill 6 of 16
 // The fragments are made in registers straight from the code words. The order of the contracted dimensions is free as long as Q has
@@ -16,15 +20,23 @@
 // it, which keep an absolute error of 2^-25 of it), and the factor returns in the softmax scale. P is held as p * 2^10 in f16, so
 // that weights down to 2^-34 of the row's largest survive. Maxima, sums and O are f32.
 //
-// Long stretches are cut into chunks (kv4_decode_chunk); each leaves its unnormalised O with maximum and sum in the workspace, and a
-// second kernel adds them up. Keys beyond the stretch are zero-filled, masked keys get p = 0.
+// A pair that lies in one CTA is finished there; the parts of one that is cut leave their unnormalised O with maximum and sum in the
+// workspace, and a second kernel adds them up in their order. Keys beyond the stretch are zero-filled, masked keys get p = 0.
 #include "common.cuh"
 #include "kv4.h"
 
 namespace kvd {
 
-constexpr int WARPS = 4, KB = 32, STAGES = 3;
+constexpr int KB = 32;
 constexpr float P_SHIFT = 10.0f;  // P is held as p * 2^10
+
+// Warps of a CTA, blocks in a warp's ring, CTAs per SM, Q fragments in shared memory instead of registers
+template <int HD, int NT> struct Cfg {
+  static constexpr int WARPS = HD == 256 && NT == 1 ? 6 : 4;
+  static constexpr int STAGES = HD == 256 && NT == 1 ? 2 : 3;
+  static constexpr int CTAS = HD == 256 ? (NT == 1 ? 2 : 1) : NT == 1 ? 3 : 2;
+  static constexpr bool Q_SMEM = NT * HD >= 256;
+};
 
 template <int HD> struct Ring {
   static constexpr int ROW = HD / 2, SROW = HD / 16;                            // bytes of a key's codes and scales
@@ -88,10 +100,11 @@ template <int HD> __device__ __forceinline__ int v_chunk(int k, int c) { return 
 
 struct Args {
   Kv4DecodeArgs a;
-  int chunk;       // keys per chunk
-  int n_chunks;    // chunks of max_len; with more than one, the parts go to the workspace
-  float* ws_o;     // [T * heads][n_chunks][hd]
-  float2* ws_ml;   // [T * heads][n_chunks] (maximum in log2 units, sum)
+  int q_min;       // least blocks per CTA
+  int max_parts;   // parts of a pair, at most: max_len in blocks / q_min, and one more for its offset
+  float* ws_o;     // [T * heads][max_parts][hd]
+  float2* ws_ml;   // [T * heads][max_parts] (maximum in log2 units, sum)
+  int* ws_n;       // [T * heads] parts of the row's pair
 };
 
 struct Sequence {
@@ -118,40 +131,117 @@ __device__ __forceinline__ Sequence sequence(const Kv4DecodeArgs& a, int b, bool
   return s;
 }
 
-// out row of head_dim values: normalised, gated, rounded once. n consecutive values of one thread.
-__device__ __forceinline__ float gated(float o, const bf16* gate, int d) {
-  return gate ? o * sigmoid_f(__bfloat162float(gate[d])) : o;
+template <int ROWS>
+__device__ __forceinline__ int rounds_of(const Sequence& s, int G) { return (s.L * G + ROWS - 1) / ROWS; }
+// Blocks of one pair of the sequence: at least one, so that the tokens of an empty stretch get their zeros.
+__device__ __forceinline__ int blocks_of(const Sequence& s) { return max(1, (s.len + KB - 1) / KB); }
+
+// PER consecutive values of a row from dimension d: normalised, gated, rounded once
+template <int PER>
+__device__ __forceinline__ void store_row(const Kv4DecodeArgs& a, const float (&acc)[PER], float sum, size_t at, int t, int h, int hd, int d) {
+  const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+  const bf16* gate = a.gate_qg ? a.gate_qg + (size_t)t * a.qg_stride + (size_t)(2 * h + 1) * hd + d : nullptr;
+  bf16* out = a.out + at * hd + d;
+#pragma unroll
+  for (int i = 0; i < PER; i += 2) {
+    float x = acc[i] * inv, y = acc[i + 1] * inv;
+    if (gate) {
+      const __nv_bfloat162 gv = *reinterpret_cast<const __nv_bfloat162*>(gate + i);
+      x *= sigmoid_f(__low2float(gv));
+      y *= sigmoid_f(__high2float(gv));
+    }
+    *reinterpret_cast<__nv_bfloat162*>(out + i) = __floats2bfloat162_rn(x, y);
+  }
 }
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(WARPS * 32, 2) kv4_decode_kernel(const Args p) {
+__global__ void __launch_bounds__(Cfg<HD, NT>::WARPS * 32, Cfg<HD, NT>::CTAS) kv4_decode_kernel(const Args p) {
   using R = Ring<HD>;
   constexpr int KW = HD / 32;               // K code words of a lane per key
   constexpr int KL = KW < 4 ? KW : 4;       // ... loaded at once
   constexpr int VW = HD / 64;               // V code words of a lane per key
   constexpr int ROWS = 8 * NT;
-  constexpr bool Q_SMEM = NT * HD > 256;    // Q fragments from shared memory where registers run out
+  constexpr int WARPS = Cfg<HD, NT>::WARPS, STAGES = Cfg<HD, NT>::STAGES;
+  constexpr bool Q_SMEM = Cfg<HD, NT>::Q_SMEM;
   const Kv4DecodeArgs& a = p.a;
-  const int b = blockIdx.z, kh = blockIdx.y, z = blockIdx.x;
-  const Sequence sq = sequence(a, b, z == 0 && kh == 0 && threadIdx.x == 0);
-  const int k0 = z * p.chunk, k1 = min(sq.len, k0 + p.chunk);  // this chunk's keys, relative to the stretch
-  if (p.n_chunks > 1 && k0 >= k1) return;                      // the merge reads only chunks that hold keys
-  const int G = a.heads / a.kv, n_rows = sq.L * G;
+  const int G = a.heads / a.kv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   extern __shared__ __align__(16) uint8_t smem[];
   uint8_t* ring = smem + warp * (STAGES * R::BYTES);
   const uint32_t ring_addr = smem_addr(ring);
   uint2* q_smem = reinterpret_cast<uint2*>(smem + WARPS * STAGES * R::BYTES);  // [word * 2 + half][nt][lane]
   const float scale_log2e = (1.0f / sqrtf((float)HD)) * 1.4426950408889634f;
-  const int n_blocks = k1 > k0 ? (k1 - k0 + KB - 1) / KB : 0;
 
-  // rows of the cache for this head
-  const size_t row0 = (sq.start + (size_t)k0) * a.kv + kh;
-  const uint8_t* kc = a.cache.k.codes + row0 * R::ROW;
-  const uint8_t* vc = a.cache.v.codes + row0 * R::ROW;
-  const uint8_t* ks = a.cache.k.scales + row0 * R::SROW;
-  const uint8_t* vs = a.cache.v.scales + row0 * R::SROW;
-  const size_t code_step = (size_t)a.kv * R::ROW, scale_step = (size_t)a.kv * R::SROW;
+  // ---- this CTA's blocks: thread t adds up the sequences [t * per, (t + 1) * per), then a scan over the threads ------------------------------
+  __shared__ long long sums[WARPS];
+  __shared__ int at_b;
+  __shared__ long long at_u;
+  long long u, u_end, quota;
+  int b;
+  {
+    const int per = (a.B + WARPS * 32 - 1) / (WARPS * 32), b0 = min((int)threadIdx.x * per, a.B), b1 = min(b0 + per, a.B);
+    long long mine = 0;
+    for (int i = b0; i < b1; ++i) {
+      const Sequence s = sequence(a, i, blockIdx.x == 0);
+      mine += (long long)a.kv * rounds_of<ROWS>(s, G) * blocks_of(s);
+    }
+    long long before = mine, total = 0;
+#pragma unroll
+    for (int i = 1; i < 32; i <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, before, i);
+      if (lane >= i) before += x;
+    }
+    if (lane == 31) sums[warp] = before;
+    before -= mine;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+      if (i < warp) before += sums[i];
+      total += sums[i];
+    }
+    quota = max((total + gridDim.x - 1) / (long long)gridDim.x, (long long)p.q_min);
+    u = quota * blockIdx.x;
+    u_end = min(total, u + quota);
+    if (u >= u_end) return;
+    if (before <= u && u < before + mine) {  // one thread: its range holds the first block
+      int i = b0;
+      for (; i < b1; ++i) {
+        const Sequence s = sequence(a, i, false);
+        const long long n = (long long)a.kv * rounds_of<ROWS>(s, G) * blocks_of(s);
+        if (u < before + n) break;
+        before += n;
+      }
+      at_b = i;
+      at_u = before;
+    }
+    __syncthreads();
+    b = at_b;
+  }
+  long long seq_u = at_u;  // first block of sequence b
+  Sequence sq = sequence(a, b, false);
+
+  while (u < u_end) {
+    const int nblk = blocks_of(sq), n_rows = sq.L * G;
+    const long long in_seq = u - seq_u;
+    if (in_seq >= (long long)a.kv * rounds_of<ROWS>(sq, G) * nblk) {
+      seq_u += (long long)a.kv * rounds_of<ROWS>(sq, G) * nblk;
+      sq = sequence(a, ++b, false);
+      continue;
+    }
+    const int pair = (int)(in_seq / nblk), kh = pair % a.kv, r0 = pair / a.kv * ROWS, first_blk = (int)(in_seq - (long long)pair * nblk);
+    const int n_blocks = (int)min((long long)(nblk - first_blk), u_end - u);
+    const long long pair_u = u - first_blk;
+    const int n_parts = (int)((pair_u + nblk - 1) / quota - pair_u / quota) + 1, part = (int)blockIdx.x - (int)(pair_u / quota);
+    u += n_blocks;
+    const int k0 = first_blk * KB, k1 = min(sq.len, k0 + n_blocks * KB);  // the keys of this part, relative to the stretch
+
+    // rows of the cache for this head
+    const size_t row0 = (sq.start + (size_t)k0) * a.kv + kh;
+    const uint8_t* kc = a.cache.k.codes + row0 * R::ROW;
+    const uint8_t* vc = a.cache.v.codes + row0 * R::ROW;
+    const uint8_t* ks = a.cache.k.scales + row0 * R::SROW;
+    const uint8_t* vs = a.cache.v.scales + row0 * R::SROW;
+    const size_t code_step = (size_t)a.kv * R::ROW, scale_step = (size_t)a.kv * R::SROW;
 
   auto fetch = [&](int blk, int slot) {
     const int j0 = blk * KB, left = (k1 - k0) - j0;  // keys of the block that exist
@@ -171,7 +261,6 @@ __global__ void __launch_bounds__(WARPS * 32, 2) kv4_decode_kernel(const Args p)
     cp_async<R::SROW>(base + R::VS + lane * R::SROW, vs + at, ok);
   };
 
-  for (int r0 = 0; r0 < n_rows; r0 += ROWS) {  // one round but for many tokens
     // ---- the first blocks are on their way before Q is read -----------------------------------------
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) {
@@ -404,9 +493,11 @@ __global__ void __launch_bounds__(WARPS * 32, 2) kv4_decode_kernel(const Args p)
     cp_wait<0>();
     __syncthreads();  // the rings are free: they take the warps' parts
 
-    // ---- the four warps' parts of each row ---------------------------------------------------------------
-    float* part_o = reinterpret_cast<float*>(smem);                       // [warp][row][HD]
-    float2* part_ml = reinterpret_cast<float2*>(smem + WARPS * ROWS * HD * 4);  // [warp][row]
+    // ---- the four warps' parts of each row. Dimension g * (HD / 8) + 2 t + e lies at t * 16 + 2 g + e, and rows are HD + 4 floats
+    // apart: the sixteen lanes of a store (four g, four rows two apart) then meet sixteen different pairs of banks ----------------
+    constexpr int PITCH = HD + 4;
+    float* part_o = reinterpret_cast<float*>(smem);                                // [warp][row][PITCH]
+    float2* part_ml = reinterpret_cast<float2*>(smem + WARPS * ROWS * PITCH * 4);  // [warp][row]
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -416,13 +507,14 @@ __global__ void __launch_bounds__(WARPS * 32, 2) kv4_decode_kernel(const Args p)
         l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], 16);
         const int row = nt * 8 + 2 * c + i;
         if (g == 0) part_ml[warp * ROWS + row] = make_float2(m[nt][i], l[nt][i]);
-        float* dst = part_o + (size_t)(warp * ROWS + row) * HD + g * (HD / 8);
+        float* dst = part_o + (warp * ROWS + row) * PITCH + 2 * g;
 #pragma unroll
-        for (int t = 0; t < HD / 16; ++t) *reinterpret_cast<float2*>(dst + 2 * t) = make_float2(o[t][nt][i], o[t][nt][i + 2]);
+        for (int t = 0; t < HD / 16; ++t) *reinterpret_cast<float2*>(dst + 16 * t) = make_float2(o[t][nt][i], o[t][nt][i + 2]);
       }
     __syncthreads();
     const int rows_here = min(ROWS, n_rows - r0);
-    constexpr int PER = HD / 32;  // values of a lane; one warp per row
+    constexpr int PER = HD / 32;  // consecutive values of a lane; one warp per row
+    const int d0 = lane * PER, at0 = d0 % (HD / 8) * 8 + d0 / (HD / 8) * 2;
     for (int row = warp; row < rows_here; row += WARPS) {
       float M = -INFINITY;
 #pragma unroll
@@ -436,22 +528,25 @@ __global__ void __launch_bounds__(WARPS * 32, 2) kv4_decode_kernel(const Args p)
         const float fw = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
         sum += fw * ml.y;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) acc[i] += fw * part_o[(size_t)(w * ROWS + row) * HD + lane + 32 * i];
+        for (int i = 0; i < PER; i += 2) {
+          const float2 v = *reinterpret_cast<const float2*>(part_o + (w * ROWS + row) * PITCH + at0 + 8 * i);
+          acc[i] += fw * v.x;
+          acc[i + 1] += fw * v.y;
+        }
       }
       const int r = r0 + row, t = sq.off + r / G, h = kh * G + r % G;
       const size_t at = (size_t)t * a.heads + h;
-      if (p.n_chunks > 1) {
-        if (lane == 0) p.ws_ml[at * p.n_chunks + z] = make_float2(M, sum);
+      if (part == 0 && lane == 0) p.ws_n[at] = n_parts;
+      if (n_parts > 1) {
+        if (lane == 0) p.ws_ml[at * p.max_parts + part] = make_float2(M, sum);
+        float* dst = p.ws_o + (at * p.max_parts + part) * HD + d0;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) p.ws_o[(at * p.n_chunks + z) * HD + lane + 32 * i] = acc[i];
+        for (int i = 0; i < PER; i += 2) *reinterpret_cast<float2*>(dst + i) = make_float2(acc[i], acc[i + 1]);
       } else {
-        const bf16* gate = a.gate_qg ? a.gate_qg + (size_t)t * a.qg_stride + (size_t)h * 2 * HD + HD : nullptr;
-        const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) a.out[at * HD + lane + 32 * i] = __float2bfloat16_rn(gated(acc[i] * inv, gate, lane + 32 * i));
+        store_row<PER>(a, acc, sum, at, t, h, HD, d0);
       }
     }
-    if (r0 + ROWS < n_rows) __syncthreads();  // before the rings are filled again
+    if (u < u_end) __syncthreads();  // before the rings are filled again
   }
 }
 
@@ -470,8 +565,9 @@ __global__ void __launch_bounds__(128) kv4_decode_merge_kernel(const Args p) {
   }
   const Sequence sq = sequence(a, lo, false);
   if (sq.L == 0) return;
-  const int nz = (sq.len + p.chunk - 1) / p.chunk;
-  const float2* ml = p.ws_ml + at * p.n_chunks;
+  const int nz = p.ws_n[at];
+  if (nz == 1) return;  // finished by its only CTA
+  const float2* ml = p.ws_ml + at * p.max_parts;
   float M = -INFINITY;
   for (int z = lane; z < nz; z += 32) M = fmaxf(M, ml[z].x);
   M = warp_max(M);
@@ -479,7 +575,7 @@ __global__ void __launch_bounds__(128) kv4_decode_merge_kernel(const Args p) {
 #pragma unroll
   for (int i = 0; i < PER; ++i) acc[i] = 0.f;
   if (M != -INFINITY) {
-    const float* src = p.ws_o + at * p.n_chunks * HD + lane * PER;
+    const float* src = p.ws_o + at * p.max_parts * HD + lane * PER;
 #pragma unroll 4
     for (int z = 0; z < nz; ++z) {
       const float2 x = ml[z];
@@ -493,13 +589,7 @@ __global__ void __launch_bounds__(128) kv4_decode_merge_kernel(const Args p) {
       }
     }
   }
-  const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-  const bf16* gate = a.gate_qg ? a.gate_qg + (size_t)t * a.qg_stride + (size_t)h * 2 * HD + HD : nullptr;
-#pragma unroll
-  for (int i = 0; i < PER; i += 2) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(gated(acc[i] * inv, gate, lane * PER + i), gated(acc[i + 1] * inv, gate, lane * PER + i + 1));
-    *reinterpret_cast<__nv_bfloat162*>(a.out + at * HD + lane * PER + i) = v;
-  }
+  store_row<PER>(a, acc, sum, at, t, h, HD, lane * PER);
 }
 
 int sm_count() {
@@ -508,47 +598,54 @@ int sm_count() {
   return sms;
 }
 
-// Keys per chunk: as long as there are eight CTAs per SM (two resident ones four times over, for the ragged tail), at most 2048 (a
-// part's O is then under 1 % of what its keys weigh) and at least 128 (a block per warp).
-int chunk_of(int B, int kv, int max_len) {
-  int chunk = 2048;
-  while (chunk > 128 && (size_t)B * kv * (((size_t)max_len + chunk - 1) / chunk) < (size_t)8 * sm_count()) chunk >>= 1;
-  return chunk;
+// The number of CTAs (two per SM are resident), the least blocks that one takes (one per warp, and not so few that the parts of a pair
+// outgrow the workspace where most sequences are far shorter than max_len), and the parts that a pair can then have.
+struct Plan {
+  int ctas, q_min, max_parts;
+};
+Plan plan_of(int B, int kv, int max_len) {
+  Plan p;
+  p.ctas = sm_count();
+  const long long blocks = max(1, (int)(((long long)max_len + KB - 1) / KB));
+  p.q_min = (int)max(4LL, ((long long)B * kv * blocks / (2 * p.ctas) + 3) / 4);
+  p.max_parts = (int)((blocks + p.q_min - 1) / p.q_min) + 1;
+  return p;
 }
 
 template <int HD, int NT>
-cudaError_t run(const Args& p, cudaStream_t s) {
-  constexpr int rings = WARPS * STAGES * Ring<HD>::BYTES, parts = WARPS * 8 * NT * (HD * 4 + 8);
-  constexpr int bytes = (rings + (NT * HD > 256 ? HD / 32 * 2 * NT * 256 : 0)) > parts ? (rings + (NT * HD > 256 ? HD / 32 * 2 * NT * 256 : 0)) : parts;
+cudaError_t run(const Args& p, int ctas, cudaStream_t s) {
+  using C = Cfg<HD, NT>;
+  constexpr int rings = C::WARPS * C::STAGES * Ring<HD>::BYTES + (C::Q_SMEM ? HD / 16 * NT * 256 : 0), parts = C::WARPS * 8 * NT * ((HD + 4) * 4 + 8);
+  constexpr int bytes = rings > parts ? rings : parts;
+  static_assert(C::CTAS * (bytes + 1024 + 256) <= 228 * 1024, "shared memory of an SM");
   CUDA_TRY(cudaFuncSetAttribute(kv4_decode_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  kv4_decode_kernel<HD, NT><<<dim3(p.n_chunks, p.a.kv, p.a.B), WARPS * 32, bytes, s>>>(p);
+  kv4_decode_kernel<HD, NT><<<ctas * C::CTAS, C::WARPS * 32, bytes, s>>>(p);
   CUDA_TRY(cudaGetLastError());
-  if (p.n_chunks > 1) {
-    const size_t rows = (size_t)p.a.T * p.a.heads;
-    kv4_decode_merge_kernel<HD><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
-  }
+  const size_t rows = (size_t)p.a.T * p.a.heads;
+  kv4_decode_merge_kernel<HD><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
   return cudaGetLastError();
 }
 
 }  // namespace kvd
 
 size_t kv4_decode_workspace(int B, int T, int max_len, int heads, int kv, int hd) {
-  const int chunk = kvd::chunk_of(B, kv, max_len);
-  const size_t n = ((size_t)max_len + chunk - 1) / chunk;
-  return n > 1 ? (size_t)T * heads * n * ((size_t)hd * sizeof(float) + sizeof(float2)) : 0;
+  const size_t rows = (size_t)T * heads, parts = (size_t)kvd::plan_of(B, kv, max_len).max_parts;
+  return rows * (parts * ((size_t)hd * sizeof(float) + sizeof(float2)) + sizeof(int));
 }
 
 cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, void* workspace, cudaStream_t s) {
-  if (a.B > 65535 || a.kv > 65535) return cudaErrorInvalidValue;
+  const kvd::Plan plan = kvd::plan_of(a.B, a.kv, a.max_len);
+  const size_t parts = (size_t)a.T * a.heads * plan.max_parts;
   kvd::Args p;
   p.a = a;
-  p.chunk = kvd::chunk_of(a.B, a.kv, a.max_len);
-  p.n_chunks = a.max_len > p.chunk ? (int)(((size_t)a.max_len + p.chunk - 1) / p.chunk) : 1;
+  p.q_min = plan.q_min;
+  p.max_parts = plan.max_parts;
   p.ws_o = (float*)workspace;
-  p.ws_ml = (float2*)((char*)workspace + (size_t)a.T * a.heads * p.n_chunks * a.hd * sizeof(float));
+  p.ws_ml = (float2*)(p.ws_o + parts * a.hd);
+  p.ws_n = (int*)(p.ws_ml + parts);
   // column tiles of eight rows by the rows of a sequence of average length; longer ones take several rounds over their keys
-  const int rows = ((a.T + a.B - 1) / a.B) * (a.heads / a.kv);
-  if (a.hd == 256) return rows <= 8 ? kvd::run<256, 1>(p, s) : kvd::run<256, 2>(p, s);
-  if (a.hd == 128) return rows <= 8 ? kvd::run<128, 1>(p, s) : rows <= 16 ? kvd::run<128, 2>(p, s) : kvd::run<128, 4>(p, s);
-  return rows <= 8 ? kvd::run<64, 1>(p, s) : rows <= 16 ? kvd::run<64, 2>(p, s) : kvd::run<64, 4>(p, s);
+  const int rows = ((a.T + a.B - 1) / a.B) * (a.heads / a.kv), n = plan.ctas;
+  if (a.hd == 256) return rows <= 8 ? kvd::run<256, 1>(p, n, s) : kvd::run<256, 2>(p, n, s);
+  if (a.hd == 128) return rows <= 8 ? kvd::run<128, 1>(p, n, s) : rows <= 16 ? kvd::run<128, 2>(p, n, s) : kvd::run<128, 4>(p, n, s);
+  return rows <= 8 ? kvd::run<64, 1>(p, n, s) : rows <= 16 ? kvd::run<64, 2>(p, n, s) : kvd::run<64, 4>(p, n, s);
 }
