@@ -14,8 +14,9 @@
 //                  grown by more than 2^8; the groups hand the maximum in use from tile to tile through shared memory.
 //   O += P V       P as the TMEM operand (over S[j]), V from shared memory, O in TMEM
 // The tensor core runs S[0], S[1], then P.V[j], S[j + 2] in turn: a tile's softmax has a whole tile's products to hide behind.
-// K (128 keys x 64 dims) and V (8192 / head_dim keys x all dims) come through one ring of 16 KB slots in the order in which they are
-// used, so that the loads run two and more product phases ahead.
+// K and V come through one ring in the order in which they are used, so that the loads run two and more product phases ahead. A slot is
+// 32 KB (16 KB at head_dim 64, a whole tile): with 16 KB slots the issuing warp, which spends 200 to 300 cycles on a slot beside its
+// products (a satisfied wait alone takes 100 to 170), was slower than the tensor core: 4360 cycles a tile of 2048 at head_dim 256.
 //
 // Keys that do not exist are never multiplied as they lie in memory: the state's map ends at its last row (zeros behind it); of the own
 // keys' last tile only steps of 16 with a key in them are multiplied, and the rows behind the last key are zeroed in shared memory
@@ -34,18 +35,19 @@ namespace kvq {
 using namespace tcc;
 
 constexpr int KT = 128;                   // keys of a tile
-constexpr uint32_t SLOT = 16384;          // bytes of a ring slot
 constexpr int NUM_THREADS = 320, ISSUER = 8, LOADER = 9;
 constexpr uint32_t S_COL = 256;           // TMEM: O from column 0, S at 256 and 384
 constexpr float RESCALE = 8.0f;           // log2 units
-constexpr uint32_t BAR_BYTES = 512, EXCHANGE_BYTES = 2 * 128 * 4 * 2;
+constexpr uint32_t BAR_BYTES = 512, M_BYTES = 2 * 128 * 4;
 
 template <int HD> struct Shape {
-  static constexpr int NKB = HD / 64;                        // K slabs of a tile, 64 dims each
-  static constexpr int KSUB = 8192 / HD;                     // keys of a V slot
+  static constexpr uint32_t SLOT = HD == 64 ? 16384 : 32768;  // bytes of a ring slot
+  static constexpr int NKB = HD / 64;                         // 64-dim slabs of Q and K
+  static constexpr int SLABS = SLOT / 16384;                  // slabs of a K slot
+  static constexpr int KSUB = SLOT / (2 * HD);                // keys of a V slot
   static constexpr uint32_t Q_BYTES = 128 * HD * 2;
-  static constexpr int SLOTS = HD == 256 ? 9 : 10;
-  static constexpr uint32_t SMEM = Q_BYTES + SLOTS * SLOT + EXCHANGE_BYTES + BAR_BYTES + 1024;
+  static constexpr int SLOTS = HD == 256 ? 5 : HD == 128 ? 6 : 10;
+  static constexpr uint32_t SMEM = Q_BYTES + SLOTS * SLOT + M_BYTES + BAR_BYTES + 1024;
   static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
 };
 
@@ -128,9 +130,9 @@ __device__ __forceinline__ bool find_tile(const Params& p, int want, bool revers
         sums[2] = (want - before) * p.tokens;
       }
       __syncthreads();
-      tile.off = sums[0];
-      tile.L = sums[1];
-      tile.t0 = sums[2];
+      tile.off = __shfl_sync(0xffffffffu, sums[0], 0);  // uniform for the compiler too: what the issuing warps compute from it stays
+      tile.L = __shfl_sync(0xffffffffu, sums[1], 0);    // on the uniform datapath (an MMA costs 60 to 75 cycles to issue otherwise, 21 so)
+      tile.t0 = __shfl_sync(0xffffffffu, sums[2], 0);
       tile.ntok = min(p.tokens, tile.L - tile.t0);
       return true;
     }
@@ -162,15 +164,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKs, const __grid_constant__ CUtensorMap tmVs,
                      const __grid_constant__ CUtensorMap tmKo, const __grid_constant__ CUtensorMap tmVo, const Params p) {
   using D = Shape<HD>;
-  constexpr int NKB = D::NKB, KSUB = D::KSUB, SLOTS = D::SLOTS;
+  constexpr int NKB = D::NKB, SLABS = D::SLABS, KSUB = D::KSUB, SLOTS = D::SLOTS;
+  constexpr uint32_t SLOT = D::SLOT;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), pad = ((raw + 1023u) & ~1023u) - raw;
   uint8_t* smem = smem_raw + pad;
   const uint32_t q_base = raw + pad, ring = q_base + D::Q_BYTES;
   float* m_used = reinterpret_cast<float*>(smem + D::Q_BYTES + SLOTS * SLOT);  // [2][128] by tile parity
-  float* l_part = m_used + 256;                                                // [2][128] by group
-  uint8_t* bars_ptr = smem + D::Q_BYTES + SLOTS * SLOT + EXCHANGE_BYTES;
-  const uint32_t bars = ring + SLOTS * SLOT + EXCHANGE_BYTES;
+  float* l_part = reinterpret_cast<float*>(smem + D::Q_BYTES);                 // [2][128] by group, over the ring, after the last product
+  uint8_t* bars_ptr = smem + D::Q_BYTES + SLOTS * SLOT + M_BYTES;
+  const uint32_t bars = ring + SLOTS * SLOT + M_BYTES;
   // by tile parity: S done, P written, P.V done, maximum published. A parity wait is sound while the barrier is at most one phase
   // behind the waiter: with two barriers that is two tiles, and nobody runs two tiles ahead of P.V (S[j] comes behind P.V[j - 2]).
   const uint32_t bar_q = bars, bar_s = bars + 8, bar_p = bars + 24, bar_o = bars + 40, bar_m = bars + 56, bar_done = bars + 72, bar_l = bars + 80;
@@ -225,7 +228,7 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_holder;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_holder, 0);
 
   if (warp == LOADER) {
     // ---- Q, then K[0], K[1], V[0], K[2], V[1], K[3] ... through the ring: the order in which the issuer uses them ------------------
@@ -245,34 +248,32 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     auto advance = [&]() {
       if (++slot == SLOTS) { slot = 0; ++use; }
     };
-    auto load_k = [&](int j) {
-      const bool st = keys.state(j);
-      const int row = keys.key0(j) + (st ? 0 : tile.off);
-      for (int c = 0; c < NKB && next_slot(); ++c) {
-        if (el) {
-          mbar_expect_tx(full + 8 * slot, SLOT);
-          tma_load_2d(ring + slot * SLOT, st ? &tmKs : &tmKo, full + 8 * slot, kh * HD + c * 64, row);
-        }
-        advance();
-      }
-    };
-    auto load_v = [&](int j) {
-      const bool st = keys.state(j);
-      const int row = keys.key0(j) + (st ? 0 : tile.off), valid = keys.valid(j, p, tile);
-      for (int s = 0; s * KSUB < valid && next_slot(); ++s) {
-        if (el) {
-          mbar_expect_tx(full + 8 * slot, SLOT);
+    for (int i = 0; i < n_tiles + 2 && ok; ++i) {
+      if (i >= 2) {
+        const int j = i - 2;
+        const bool st = keys.state(j);
+        const int row = keys.key0(j) + (st ? 0 : tile.off), valid = keys.valid(j, p, tile);
+        for (int s = 0; s * KSUB < valid && next_slot(); ++s) {
+          if (el) {
+            mbar_expect_tx(full + 8 * slot, SLOT);
 #pragma unroll
-          for (int c = 0; c < NKB; ++c) tma_load_2d(ring + slot * SLOT + c * (KSUB * 128), st ? &tmVs : &tmVo, full + 8 * slot, kh * HD + c * 64, row + s * KSUB);
+            for (int c = 0; c < NKB; ++c) tma_load_2d(ring + slot * SLOT + c * (KSUB * 128), st ? &tmVs : &tmVo, full + 8 * slot, kh * HD + c * 64, row + s * KSUB);
+          }
+          advance();
         }
-        advance();
       }
-    };
-    load_k(0);
-    if (ok && n_tiles > 1) load_k(1);
-    for (int j = 0; j < n_tiles && ok; ++j) {
-      load_v(j);
-      if (ok && j + 2 < n_tiles) load_k(j + 2);
+      if (i < n_tiles) {
+        const bool st = keys.state(i);
+        const int row = keys.key0(i) + (st ? 0 : tile.off);
+        for (int s = 0; s < NKB / SLABS && ok && next_slot(); ++s) {
+          if (el) {
+            mbar_expect_tx(full + 8 * slot, SLOT);
+#pragma unroll
+            for (int c = 0; c < SLABS; ++c) tma_load_2d(ring + slot * SLOT + c * 16384, st ? &tmKs : &tmKo, full + 8 * slot, kh * HD + (s * SLABS + c) * 64, row);
+          }
+          advance();
+        }
+      }
     }
   } else if (warp == ISSUER) {
     const bool el = elect_one();
@@ -287,53 +288,66 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     auto advance = [&]() {
       if (++slot == SLOTS) { slot = 0; ++use; }
     };
-    auto issue_s = [&](int j) {
-      const int n = (keys.valid(j, p, tile) + 15) & ~15;  // columns that hold a key
-      const uint32_t idesc = umma_idesc(128, 0, 0) | ((uint32_t)(n >> 3) << 17);
-      const uint32_t d = tmem + S_COL + (j & 1) * KT;
-      for (int c = 0; c < NKB && wait_slot(); ++c) {
-        const uint64_t dq = umma_desc(q_base + c * 16384, 16, 1024), dk = umma_desc(ring + slot * SLOT, 16, 1024);
-        if (el) {
+    for (int i = 0; i < n_tiles + 2 && ok; ++i) {
+      if (i >= 2) {  // O += P[j] V[j]; P[j] lies over S[j]: 16 keys = 8 columns of bf16 pairs
+        const int j = i - 2;
+        if (!(ok = mbar_wait_warp(bar_p + 8 * (j & 1), (uint32_t)((j >> 1) & 1), abort_flag))) break;
+        tc_fence_after();
+        const int valid = keys.valid(j, p, tile);
+        constexpr uint32_t idesc = umma_idesc(128, HD, 1);
+        const uint32_t pj = tmem + S_COL + (j & 1) * KT;
+        for (int s = 0; s * KSUB < valid && wait_slot(); ++s) {
+          const int left = valid - s * KSUB;
+          const uint64_t dv = umma_desc(ring + slot * SLOT, KSUB * 128, 1024);
+          if (left >= KSUB) {
+            if (el) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_f16(d, dq + (uint64_t)(k * 2), dk + (uint64_t)(k * 2), idesc, (c | k) != 0 ? 1u : 0u);
-          umma_commit_to(empty + 8 * slot);
-        }
-        advance();
-      }
-      if (ok && el) umma_commit_to(bar_s + 8 * (j & 1));
-    };
-    if (ok) issue_s(0);
-    if (ok && n_tiles > 1) issue_s(1);
-    for (int j = 0; j < n_tiles && ok; ++j) {
-      if (!(ok = mbar_wait_warp(bar_p + 8 * (j & 1), (uint32_t)((j >> 1) & 1), abort_flag))) break;
-      tc_fence_after();
-      const int valid = keys.valid(j, p, tile);
-      constexpr uint32_t idesc = umma_idesc(128, HD, 1);
-      for (int s = 0; s * KSUB < valid && wait_slot(); ++s) {
-        const int left = min(valid - s * KSUB, KSUB), steps = (left + 15) >> 4;
-        if (left & 15) {  // rows behind the last key of the step
-          const int rows = steps * 16 - left;
-          for (int i = lane; i < rows * NKB * 8; i += 32) {
-            const int r = i / (NKB * 8), c = i - r * (NKB * 8);
-            *reinterpret_cast<uint4*>(smem + D::Q_BYTES + slot * SLOT + (c >> 3) * (KSUB * 128) + (left + r) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+              for (int k = 0; k < KSUB / 16; ++k) umma_f16_ts(tmem, pj + (s * (KSUB / 16) + k) * 8, dv + (uint64_t)(k * 128), idesc, (j | s | k) != 0 ? 1u : 0u);
+              umma_commit_to(empty + 8 * slot);
+            }
+          } else {
+            const int steps = (left + 15) >> 4;
+            if (left & 15) {  // rows behind the last key of the step
+              const int rows = steps * 16 - left;
+              for (int z = lane; z < rows * NKB * 8; z += 32) {
+                const int r = z / (NKB * 8), c = z - r * (NKB * 8);
+                *reinterpret_cast<uint4*>(smem + D::Q_BYTES + slot * SLOT + (c >> 3) * (KSUB * 128) + (left + r) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+            }
+            if (el) {
+              for (int k = 0; k < steps; ++k) umma_f16_ts(tmem, pj + (s * (KSUB / 16) + k) * 8, dv + (uint64_t)(k * 128), idesc, (j | s | k) != 0 ? 1u : 0u);
+              umma_commit_to(empty + 8 * slot);
+            }
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
+          advance();
         }
-        const uint64_t dv = umma_desc(ring + slot * SLOT, KSUB * 128, 1024);
+        if (!ok) break;
         if (el) {
-          for (int k = 0; k < steps; ++k)  // P[j] lies over S[j]: 16 keys = 8 columns of bf16 pairs
-            umma_f16_ts(tmem, tmem + S_COL + (j & 1) * KT + (s * (KSUB / 16) + k) * 8, dv + (uint64_t)(k * (16 * 128 / 16)), idesc, (j | s | k) != 0 ? 1u : 0u);
-          umma_commit_to(empty + 8 * slot);
+          umma_commit_to(bar_o + 8 * (j & 1));
+          if (j + 1 == n_tiles) umma_commit_to(bar_done);
         }
-        advance();
       }
-      if (!ok) break;
-      if (el) {
-        umma_commit_to(bar_o + 8 * (j & 1));
-        if (j + 1 == n_tiles) umma_commit_to(bar_done);
+      if (i < n_tiles) {  // S[i]
+        const int valid = keys.valid(i, p, tile);
+        const uint32_t d = tmem + S_COL + (i & 1) * KT;
+        // a partial tile: the columns that hold a key, rounded up to the instruction's 16
+        const uint32_t idesc = valid == KT ? umma_idesc(128, KT, 0) : umma_idesc(128, 0, 0) | ((uint32_t)((valid + 15) >> 4) << 18);
+        for (int s = 0; s < NKB / SLABS && wait_slot(); ++s) {
+          if (el) {
+#pragma unroll
+            for (int c = 0; c < SLABS; ++c) {
+              const uint64_t dq = umma_desc(q_base + (s * SLABS + c) * 16384, 16, 1024), dk = umma_desc(ring + slot * SLOT + c * 16384, 16, 1024);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) umma_f16(d, dq + (uint64_t)(k * 2), dk + (uint64_t)(k * 2), idesc, (s | c | k) != 0 ? 1u : 0u);
+            }
+            umma_commit_to(empty + 8 * slot);
+          }
+          advance();
+        }
+        if (ok && el) umma_commit_to(bar_s + 8 * (i & 1));
       }
-      if (j + 2 < n_tiles) issue_s(j + 2);
     }
   } else {
     // ---- softmax: group h takes the tiles of its parity; thread r of a group has row r ----------------------------------------------
@@ -412,22 +426,29 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       mbar_arrive(bar_p + 8 * h);
     }
     // ---- epilogue: either group takes half of the head's dimensions --------------------------------------------------------------
-    const int last = (n_tiles - 1) & 1;
+    const int last = (n_tiles - 1) & 1, tt = r / G, head = head0 + r - tt * G;
+    const bool live = tt < tile.ntok;
+    const size_t t = (size_t)tile.off + tile.t0 + tt;
+    const bf16* gate = p.gate_qg && live && gridDim.z == 1 ? p.gate_qg + t * p.qg_stride + (size_t)(2 * head + 1) * HD + h * (HD / 2) : nullptr;
+    uint4 gv[HD / 16];  // on their way while the last product runs
+    if (gate) {
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) gv[i] = *reinterpret_cast<const uint4*>(gate + i * 8);
+    }
     if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar_m + 8 * last, (uint32_t)(((n_tiles - 1) >> 1) & 1), abort_flag));
     float end_m = -INFINITY;
     if (ok) {
       end_m = m_used[last * 128 + r];
+      ok = __all_sync(0xffffffffu, mbar_wait(bar_done, 0, abort_flag));
+    }
+    if (ok) {
       l_part[h * 128 + r] = m == -INFINITY ? 0.f : l * ex2(m - end_m);
       mbar_arrive(bar_l);
       ok = __all_sync(0xffffffffu, mbar_wait(bar_l, 0, abort_flag));
     }
-    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar_done, 0, abort_flag));
     if (ok) {
       tc_fence_after();
       const float sum = l_part[r] + l_part[128 + r];
-      const int tt = r / G, head = head0 + r - tt * G;
-      const bool live = tt < tile.ntok;
-      const size_t t = (size_t)tile.off + tile.t0 + tt;
       if (gridDim.z > 1) {
         if (h == 0) p.ws_ml[block_lin * 128 + r] = make_float2(end_m, sum);
         float* dst = p.ws_o + (block_lin * 128 + r) * HD;
@@ -443,17 +464,11 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         }
       } else {
         const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-        const bf16* gate = p.gate_qg && live ? p.gate_qg + t * p.qg_stride + (size_t)(2 * head + 1) * HD : nullptr;
-        bf16* dst = p.out + (t * p.heads + head) * HD;
-#pragma unroll 1
-        for (int c = h * (HD / 2); c < (h + 1) * (HD / 2); c += 32) {
-          uint32_t v[32];
-          uint4 gv[4];
-          tmem_ld32(tmem + lanes + c, v);
-          if (gate) {
+        bf16* dst = p.out + (t * p.heads + head) * HD + h * (HD / 2);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) gv[i] = *reinterpret_cast<const uint4*>(gate + c + i * 8);
-          }
+        for (int c = 0; c < HD / 2; c += 32) {
+          uint32_t v[32];
+          tmem_ld32(tmem + lanes + h * (HD / 2) + c, v);
           tmem_ld_wait();
           if (live) {
 #pragma unroll
@@ -462,7 +477,7 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
               for (int k = 0; k < 8; ++k) o[k] = __uint_as_float(v[i * 8 + k]) * inv;
               if (gate) {
-                const __nv_bfloat162* g2 = reinterpret_cast<const __nv_bfloat162*>(&gv[i]);
+                const __nv_bfloat162* g2 = reinterpret_cast<const __nv_bfloat162*>(&gv[c / 8 + i]);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                   o[2 * k] *= __fdividef(1.0f, 1.0f + __expf(-__low2float(g2[k])));
