@@ -5,18 +5,24 @@
 // into the workspace, 2 x n_state x kv x head_dim x 2 bytes that mostly stay in L2, and the attention reads state and own keys alike
 // through TMA.
 //
-// One CTA = (question, K/V head, tile of 128 / G tokens): the G query heads of a K/V head share its keys, so the 128 rows of an MMA
-// tile are (token, head) pairs, brought in by a 3-D TMA box. Keys come in tiles of 128, the state's first, then the question's own:
+// A work item = (question, tile of 128 / G tokens, K/V head): the G query heads of a K/V head share its keys, so the 128 rows of an MMA
+// tile are (token, head) pairs, brought in by a 3-D TMA box. One CTA per SM goes through its items one after the other; the loads and
+// the first S products of an item run while the rows of the item before it are still being written. Keys come in tiles of 128, the
+// state's first, then the question's own:
 //   S = Q K^T      tcgen05.mma, both operands from shared memory, S[j] in one of two 128-column TMEM buffers
 //   P = softmax    of S[j]: one thread per row and two groups of four warps, one for even, one for odd tiles. While one group is in its
 //                  exponentials the other is in the barriers, TMEM loads and stores around its own, so neither unit waits for a
 //                  round trip, and no row is split between threads. Rescaling is lazy: O is rescaled only when a row's maximum has
 //                  grown by more than 2^8; the groups hand the maximum in use from tile to tile through shared memory.
 //   O += P V       P as the TMEM operand (over S[j]), V from shared memory, O in TMEM
-// The tensor core runs S[0], S[1], then P.V[j], S[j + 2] in turn: a tile's softmax has a whole tile's products to hide behind.
-// K and V come through one ring in the order in which they are used, so that the loads run two and more product phases ahead. A slot is
-// 32 KB (16 KB at head_dim 64, a whole tile): with 16 KB slots the issuing warp, which spends 200 to 300 cycles on a slot beside its
-// products (a satisfied wait alone takes 100 to 170), was slower than the tensor core: 4360 cycles a tile of 2048 at head_dim 256.
+// The tensor core runs S[0], S[1], then P.V[j], S[j + 2] in turn, so a tile's softmax has a whole tile's products to hide behind. (With
+// a second issuing warp S[j + 2] and P.V[j + 1] share the tensor core, and the loop S, softmax, P.V of a tile gets longer by that:
+// slower.) K and V come through one ring of 32 KB slots (16 KB at head_dim 64, a whole tile) in the order in which they are used, so that
+// the loads run two and more product phases ahead. A barrier wait that is already satisfied still takes 100 to 170 cycles, which made
+// the issuing warp slower than the tensor core (2048 cycles a tile at head_dim 256: 4360 with 16 KB slots, 3080 with 32 KB), so it asks
+// for the next barrier's state before it issues the products of the present one.
+// The rows of O leave through a ring slot too: lane = row in TMEM, and sixteen bytes a row would be 32 lines a store; staged, a
+// store covers four rows of 64 bytes.
 //
 // Keys that do not exist are never multiplied as they lie in memory: the state's map ends at its last row (zeros behind it); of the own
 // keys' last tile only steps of 16 with a key in them are multiplied, and the rows behind the last key are zeroed in shared memory
@@ -36,9 +42,10 @@ using namespace tcc;
 
 constexpr int KT = 128;                   // keys of a tile
 constexpr int NUM_THREADS = 320, ISSUER = 8, LOADER = 9;
+constexpr int MAX_ITEMS = 64;             // work items of a CTA
 constexpr uint32_t S_COL = 256;           // TMEM: O from column 0, S at 256 and 384
 constexpr float RESCALE = 8.0f;           // log2 units
-constexpr uint32_t BAR_BYTES = 512, M_BYTES = 2 * 128 * 4;
+constexpr uint32_t BAR_BYTES = 512, ROW_BYTES = 4 * 128 * 4, TABLE_BYTES = MAX_ITEMS * 8;
 
 template <int HD> struct Shape {
   static constexpr uint32_t SLOT = HD == 64 ? 16384 : 32768;  // bytes of a ring slot
@@ -47,7 +54,8 @@ template <int HD> struct Shape {
   static constexpr int KSUB = SLOT / (2 * HD);                // keys of a V slot
   static constexpr uint32_t Q_BYTES = 128 * HD * 2;
   static constexpr int SLOTS = HD == 256 ? 5 : HD == 128 ? 6 : 10;
-  static constexpr uint32_t SMEM = Q_BYTES + SLOTS * SLOT + M_BYTES + BAR_BYTES + 1024;
+  static constexpr int KP = NKB / SLABS, VP = KT / KSUB;      // slots of a tile's K and V
+  static constexpr uint32_t SMEM = Q_BYTES + SLOTS * SLOT + ROW_BYTES + BAR_BYTES + TABLE_BYTES;
   static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
 };
 
@@ -55,6 +63,13 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// sigmoid with the hardware exponential and reciprocal (2 ulp or so in f32; the product is rounded to bf16)
+__device__ __forceinline__ float gate_of(float g) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(g * -1.4426950408889634f)));
+  return r;
 }
 
 struct Params {
@@ -67,7 +82,8 @@ struct Params {
   bf16* out;
   float scale_log2e;
   int* err;
-  float* ws_o;     // gridDim.z > 1: unnormalised O [part][row block][row][HD], row block = blockIdx.y * gridDim.x + tile
+  int parts, max_tiles;
+  float* ws_o;     // parts > 1: unnormalised O [part][heads' tile][token tile][row][HD]
   float2* ws_ml;   // (maximum in log2 units, sum)
 };
 
@@ -75,40 +91,29 @@ struct Tile {
   int off, L, t0, ntok;  // the question's first packed row and length; the tile's first token and its tokens
 };
 
-// The question and tokens of tile `want`, counted from the last one when `reverse` (a causal prompt's late tiles are its longest, and
-// start first). Offsets are clamped to the batch, so that bad ones cannot lead outside it. All threads of the block take part;
-// `sums` holds 2 + blockDim.x / 32 ints. False: there is no such tile.
-__device__ __forceinline__ bool find_tile(const Params& p, int want, bool reverse, int* sums, Tile& tile) {
-  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, nw = nt >> 5;
-  auto tiles_of = [&](int i, int& off, int& len) {
+// Token tiles of sequence i, its offset and length. Offsets that leave the batch count as an empty sequence.
+__device__ __forceinline__ int tiles_of(const Params& p, int i, int& off, int& len) {
+  off = p.cu[i];
+  const int end = p.cu[i + 1];
+  if (off < 0 || end < off || end > p.T) {
+    set_err(p.err, DERR_OFFSETS);
     off = len = 0;
-    if (i >= p.B) return 0;
-    off = p.cu[i];
-    const int end = p.cu[i + 1];
-    if (off < 0 || end < off || end > p.T) {
-      set_err(p.err, DERR_OFFSETS);
-      off = 0;
-      return 0;
-    }
-    len = end - off;
-    return (len + p.tokens - 1) / p.tokens;
-  };
-  if (reverse) {
-    int mine = 0, off, len;
-    for (int i = tid; i < p.B; i += nt) mine += tiles_of(i, off, len);
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) sums[warp] = mine;
-    __syncthreads();
-    int total = 0;
-    for (int i = 0; i < nw; ++i) total += sums[i];
-    want = total - 1 - want;
-    __syncthreads();
-    if (want < 0) return false;
+    return 0;
   }
+  len = end - off;
+  return (len + p.tokens - 1) / p.tokens;
+}
+
+// Calls found(sequence, its tiles before it, its tiles) for every sequence, each in one thread of the block, and returns the number of
+// all tiles. `sums` holds an int per warp.
+template <typename F>
+__device__ __forceinline__ int scan_tiles(const Params& p, int* sums, F found) {
+  const int nt = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = nt >> 5;
   int base = 0;
   for (int b0 = 0; b0 < p.B; b0 += nt) {
+    const int i = b0 + (int)threadIdx.x;
     int off, len;
-    const int n = tiles_of(b0 + tid, off, len);
+    const int n = i < p.B ? tiles_of(p, i, off, len) : 0;
     int incl = n;
     for (int o = 1; o < 32; o <<= 1) {
       const int x = __shfl_up_sync(0xffffffffu, incl, o);
@@ -117,28 +122,15 @@ __device__ __forceinline__ bool find_tile(const Params& p, int want, bool revers
     if (lane == 31) sums[warp] = incl;
     __syncthreads();
     int before = base, all = base;
-    for (int i = 0; i < nw; ++i) {
-      if (i < warp) before += sums[i];
-      all += sums[i];
+    for (int w = 0; w < nw; ++w) {
+      if (w < warp) before += sums[w];
+      all += sums[w];
     }
     __syncthreads();
-    if (want < all) {
-      before += incl - n;
-      if (want >= before && want < before + n) {
-        sums[0] = off;
-        sums[1] = len;
-        sums[2] = (want - before) * p.tokens;
-      }
-      __syncthreads();
-      tile.off = __shfl_sync(0xffffffffu, sums[0], 0);  // uniform for the compiler too: what the issuing warps compute from it stays
-      tile.L = __shfl_sync(0xffffffffu, sums[1], 0);    // on the uniform datapath (an MMA costs 60 to 75 cycles to issue otherwise, 21 so)
-      tile.t0 = __shfl_sync(0xffffffffu, sums[2], 0);
-      tile.ntok = min(p.tokens, tile.L - tile.t0);
-      return true;
-    }
+    if (n > 0) found(i, before + incl - n, n);
     base = all;
   }
-  return false;
+  return base;
 }
 
 // The key tiles of a CTA: tiles [lo, lo + n) of the state's followed by the own ones (causal: as far as the tile's last token).
@@ -159,52 +151,99 @@ struct Keys {
   }
 };
 
+// Whether the phase of that parity is complete, without waiting.
+__device__ __forceinline__ uint32_t mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
+
+// Predicated instructions: a branch around each of a lane's rows costs more than the access
+__device__ __forceinline__ uint2 ld_global_if(const void* p, bool there) {
+  uint2 v;
+  asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %3, 0;\nmov.b32 %0, 0;\nmov.b32 %1, 0;\n@q ld.global.v2.b32 {%0, %1}, [%2];\n}"
+               : "=&r"(v.x), "=&r"(v.y)
+               : "l"(p), "r"((int)there));
+  return v;
+}
+__device__ __forceinline__ void st_global_if(void* p, uint2 v, bool there) {
+  asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %3, 0;\n@q st.global.v2.b32 [%0], {%1, %2};\n}" ::"l"(p), "r"(v.x), "r"(v.y), "r"((int)there) : "memory");
+}
+
+// What a work item is: its tokens, heads, part and keys. Every role goes through the same items; n_tiles == 0 (more parts than key tiles)
+// leaves one out.
+struct Item {
+  Tile tile;
+  int hg, kh, head0, z, ti;
+  __device__ __forceinline__ Item(const Params& p, const int2* table, int k, int total) {
+    const int nh = p.kv * p.sub, w = (int)blockIdx.x + k * (int)gridDim.x, rest = w / nh;
+    hg = w - rest * nh;
+    z = rest / total;
+    ti = rest - z * total;
+    if (p.causal) ti = total - 1 - ti;  // a causal prompt's late tiles are its longest: they start first
+    // uniform for the compiler too, so that what the issuing warps compute from it stays on the uniform datapath
+    const int b = __shfl_sync(0xffffffffu, table[k].x, 0);
+    tile.t0 = __shfl_sync(0xffffffffu, table[k].y, 0);
+    tile.off = p.cu[b];
+    tile.L = p.cu[b + 1] - tile.off;
+    tile.ntok = min(p.tokens, tile.L - tile.t0);
+    kh = hg / p.sub;
+    head0 = kh * (p.heads / p.kv) + (hg - kh * p.sub) * p.G;
+  }
+};
+
 template <int HD>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKs, const __grid_constant__ CUtensorMap tmVs,
                      const __grid_constant__ CUtensorMap tmKo, const __grid_constant__ CUtensorMap tmVo, const Params p) {
   using D = Shape<HD>;
-  constexpr int NKB = D::NKB, SLABS = D::SLABS, KSUB = D::KSUB, SLOTS = D::SLOTS;
+  constexpr int NKB = D::NKB, SLABS = D::SLABS, KSUB = D::KSUB, SLOTS = D::SLOTS, KP = D::KP, VP = D::VP;
   constexpr uint32_t SLOT = D::SLOT;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw = smem_u32(smem_raw), pad = ((raw + 1023u) & ~1023u) - raw;
-  uint8_t* smem = smem_raw + pad;
-  const uint32_t q_base = raw + pad, ring = q_base + D::Q_BYTES;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t q_base = smem_u32(smem), ring = q_base + D::Q_BYTES;
   float* m_used = reinterpret_cast<float*>(smem + D::Q_BYTES + SLOTS * SLOT);  // [2][128] by tile parity
-  float* l_part = reinterpret_cast<float*>(smem + D::Q_BYTES);                 // [2][128] by group, over the ring, after the last product
-  uint8_t* bars_ptr = smem + D::Q_BYTES + SLOTS * SLOT + M_BYTES;
-  const uint32_t bars = ring + SLOTS * SLOT + M_BYTES;
-  // by tile parity: S done, P written, P.V done, maximum published. A parity wait is sound while the barrier is at most one phase
-  // behind the waiter: with two barriers that is two tiles, and nobody runs two tiles ahead of P.V (S[j] comes behind P.V[j - 2]).
-  const uint32_t bar_q = bars, bar_s = bars + 8, bar_p = bars + 24, bar_o = bars + 40, bar_m = bars + 56, bar_done = bars + 72, bar_l = bars + 80;
-  const uint32_t full = bars + 96, empty = full + 8 * SLOTS;
-  static_assert(96 + 16 * SLOTS + 64 <= BAR_BYTES, "barrier area");
+  float* l_part = m_used + 256;                                                // [2][128] by group
+  uint8_t* bars_ptr = smem + D::Q_BYTES + SLOTS * SLOT + ROW_BYTES;
+  int2* table = reinterpret_cast<int2*>(bars_ptr + BAR_BYTES);                 // (sequence, first token) of the CTA's items
+  const uint32_t bars = ring + SLOTS * SLOT + ROW_BYTES;
+  // by tile parity: S done, P written, P.V done, maximum published. Tiles are counted through all items of the CTA. A parity wait is
+  // sound while the barrier is at most one phase behind the waiter: with two barriers that is two tiles, and nobody runs two tiles
+  // ahead of P.V (S[j] comes behind P.V[j - 2]). Once per item: Q loaded, Q no longer needed, last P.V done, sums exchanged, O read, the
+  // epilogue's slot free.
+  const uint32_t bar_s = bars, bar_p = bars + 16, bar_o = bars + 32, bar_m = bars + 48;
+  const uint32_t bar_q = bars + 64, bar_q_free = bars + 72, bar_done = bars + 80, bar_l = bars + 88, bar_o_free = bars + 96, bar_e = bars + 104;
+  const uint32_t full = bars + 112, empty = full + 8 * SLOTS;
+  static_assert(112 + 16 * SLOTS + 64 <= BAR_BYTES, "barrier area");
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars_ptr + BAR_BYTES - 64);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars_ptr + BAR_BYTES - 60);
-  int* sums = reinterpret_cast<int*>(bars_ptr + BAR_BYTES - 56);  // 12 ints
+  int* sums = reinterpret_cast<int*>(bars_ptr + BAR_BYTES - 56);
 
   const int warp = uniform_warp_idx(), lane = threadIdx.x & 31;
-  Tile tile;
-  if (!find_tile(p, blockIdx.x, p.causal != 0, sums, tile)) return;
-  const int G = p.G, hg = blockIdx.y, kh = hg / p.sub, head0 = kh * (p.heads / p.kv) + (hg - kh * p.sub) * G;
-  const Keys keys(p, tile, blockIdx.z, gridDim.z);
-  const int n_tiles = keys.n;
-  const size_t block_lin = ((size_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
-  if (n_tiles == 0) {  // more parts than key tiles
-    if (threadIdx.x < 128) p.ws_ml[block_lin * 128 + threadIdx.x] = make_float2(-INFINITY, 0.f);
+  if (q_base & 1023u) {  // the swizzled tiles need it; dynamic shared memory starts there as long as the kernel has no static
+    if (threadIdx.x == 0) set_err(p.err, DERR_ATTN_TIMEOUT);
     return;
   }
-
   if (threadIdx.x == 0) {
-    mbar_init(bar_q, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar_s + 8 * i, 1);
       mbar_init(bar_p + 8 * i, 128);
       mbar_init(bar_o + 8 * i, 1);
       mbar_init(bar_m + 8 * i, 128);
     }
+    mbar_init(bar_q, 1);
+    mbar_init(bar_q_free, 1);
     mbar_init(bar_done, 1);
     mbar_init(bar_l, 256);
+    mbar_init(bar_o_free, 256);
+    mbar_init(bar_e, 256);
     for (int i = 0; i < SLOTS; ++i) {
       mbar_init(full + 8 * i, 1);
       mbar_init(empty + 8 * i, 1);
@@ -212,6 +251,7 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  const int G = p.G;
   // rows behind the last (token, head) pair are never written by TMA: zeros, so that they stay finite
   {
     const int row0 = p.tokens * G, nz = (128 - row0) * 8;
@@ -225,169 +265,258 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  // the items: first the number of all tiles, then where each of this CTA's tiles lies
+  int total = scan_tiles(p, sums, [](int, int, int) {});
+  total = __shfl_sync(0xffffffffu, total, 0);
+  const int nh = p.kv * p.sub, all_items = total * nh * p.parts;
+  const int n_items = min(MAX_ITEMS, ((int)blockIdx.x < all_items ? (all_items - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0));
+  int* wanted = reinterpret_cast<int*>(l_part);  // the items' tile numbers; the rows' sums come here later
+  if ((int)threadIdx.x < n_items) {
+    const int ti = ((int)blockIdx.x + (int)threadIdx.x * (int)gridDim.x) / nh % total;
+    wanted[threadIdx.x] = p.causal ? total - 1 - ti : ti;
+  }
+  __syncthreads();
+  scan_tiles(p, sums, [&](int b, int before, int n) {
+    for (int k = 0; k < n_items; ++k)
+      if (wanted[k] >= before && wanted[k] < before + n) table[k] = make_int2(b, (wanted[k] - before) * p.tokens);
+  });
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_holder, 0);
 
   if (warp == LOADER) {
-    // ---- Q, then K[0], K[1], V[0], K[2], V[1], K[3] ... through the ring: the order in which the issuer uses them ------------------
+    // ---- per item Q, then K[0], K[1], V[0], K[2], V[1], K[3] ... through the ring: the order in which the issuer uses them; behind
+    // the last V one slot for the epilogue --------------------------------------------------------------------------------------
     const bool el = elect_one();
-    if (el) {
-      mbar_expect_tx(bar_q, (uint32_t)(NKB * p.tokens * G * 128));
-#pragma unroll
-      for (int c = 0; c < NKB; ++c) tma_load_3d(q_base + c * 16384, &tmQ, bar_q, c * 64, head0, tile.off + tile.t0);
-    }
     bool ok = true;
-    int slot = 0;
-    uint32_t use = 0;  // rounds of the ring
+    int slot = 0, live = 0, e_slot = -1;
+    uint32_t use = 0, e_parity = 0;  // use: rounds of the ring
+    auto epilogue_done = [&]() {  // the slot that the epilogue of item live - 1 or the one before it was given
+      if (ok && e_slot >= 0) ok = mbar_wait_warp(bar_e, e_parity, abort_flag);
+      e_slot = -1;
+    };
     auto next_slot = [&]() {
       if (use > 0) ok = mbar_wait_warp(empty + 8 * slot, (use - 1) & 1, abort_flag);
+      if (slot == e_slot) epilogue_done();
       return ok;
     };
     auto advance = [&]() {
       if (++slot == SLOTS) { slot = 0; ++use; }
     };
-    for (int i = 0; i < n_tiles + 2 && ok; ++i) {
-      if (i >= 2) {
-        const int j = i - 2;
-        const bool st = keys.state(j);
-        const int row = keys.key0(j) + (st ? 0 : tile.off), valid = keys.valid(j, p, tile);
-        for (int s = 0; s * KSUB < valid && next_slot(); ++s) {
-          if (el) {
-            mbar_expect_tx(full + 8 * slot, SLOT);
+    for (int k = 0; k < n_items && ok; ++k) {
+      const Item it(p, table, k, total);
+      const Keys keys(p, it.tile, it.z, p.parts);
+      if (keys.n == 0) continue;
+      if (live > 0 && !(ok = mbar_wait_warp(bar_q_free, (uint32_t)(live - 1) & 1, abort_flag))) break;
+      if (el) {
+        mbar_expect_tx(bar_q, (uint32_t)(NKB * p.tokens * G * 128));
 #pragma unroll
-            for (int c = 0; c < NKB; ++c) tma_load_2d(ring + slot * SLOT + c * (KSUB * 128), st ? &tmVs : &tmVo, full + 8 * slot, kh * HD + c * 64, row + s * KSUB);
+        for (int c = 0; c < NKB; ++c) tma_load_3d(q_base + c * 16384, &tmQ, bar_q, c * 64, it.head0, it.tile.off + it.tile.t0);
+      }
+      for (int i = 0; i < keys.n + 2 && ok; ++i) {
+        if (i >= 2) {
+          const bool st = keys.state(i - 2);
+          const int row = keys.key0(i - 2) + (st ? 0 : it.tile.off);
+          for (int s = 0; s < VP && next_slot(); ++s) {
+            if (el) {
+              mbar_expect_tx(full + 8 * slot, SLOT);
+#pragma unroll
+              for (int c = 0; c < NKB; ++c) tma_load_2d(ring + slot * SLOT + c * (KSUB * 128), st ? &tmVs : &tmVo, full + 8 * slot, it.kh * HD + c * 64, row + s * KSUB);
+            }
+            advance();
           }
-          advance();
+        }
+        if (i < keys.n) {
+          const bool st = keys.state(i);
+          const int row = keys.key0(i) + (st ? 0 : it.tile.off);
+          for (int s = 0; s < KP && ok && next_slot(); ++s) {
+            if (el) {
+              mbar_expect_tx(full + 8 * slot, SLOT);
+#pragma unroll
+              for (int c = 0; c < SLABS; ++c) tma_load_2d(ring + slot * SLOT + c * 16384, st ? &tmKs : &tmKo, full + 8 * slot, it.kh * HD + (s * SLABS + c) * 64, row);
+            }
+            advance();
+          }
         }
       }
-      if (i < n_tiles) {
-        const bool st = keys.state(i);
-        const int row = keys.key0(i) + (st ? 0 : tile.off);
-        for (int s = 0; s < NKB / SLABS && ok && next_slot(); ++s) {
-          if (el) {
-            mbar_expect_tx(full + 8 * slot, SLOT);
-#pragma unroll
-            for (int c = 0; c < SLABS; ++c) tma_load_2d(ring + slot * SLOT + c * 16384, st ? &tmKs : &tmKo, full + 8 * slot, kh * HD + (s * SLABS + c) * 64, row);
-          }
-          advance();
-        }
+      // The epilogue's slot is announced as full at once and, to keep its barriers in step, as empty too: what holds it is bar_e. One at
+      // a time, so that bar_e is never two phases ahead of this warp.
+      epilogue_done();
+      if (!ok || !next_slot()) break;
+      if (el) {
+        mbar_arrive(full + 8 * slot);
+        mbar_arrive(empty + 8 * slot);
       }
+      e_slot = slot;
+      e_parity = (uint32_t)live & 1;
+      advance();
+      ++live;
     }
   } else if (warp == ISSUER) {
     const bool el = elect_one();
-    bool ok = mbar_wait_warp(bar_q, 0, abort_flag);
-    int slot = 0;
+    bool ok = true;
+    int slot = 0, live = 0, jj = 0;  // jj: tiles of the items before
     uint32_t use = 0;
+    uint32_t early = 0;  // whether the next slot was full when it was asked for, in front of the products of the one before it
     auto wait_slot = [&]() {
-      ok = mbar_wait_warp(full + 8 * slot, use & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, early != 0) || mbar_wait_warp(full + 8 * slot, use & 1, abort_flag);
       if (ok) tc_fence_after();
       return ok;
+    };
+    auto ask_next = [&]() {
+      const bool wrap = slot + 1 == SLOTS;
+      early = mbar_test(full + 8 * (wrap ? 0 : slot + 1), (use + (wrap ? 1 : 0)) & 1);
     };
     auto advance = [&]() {
       if (++slot == SLOTS) { slot = 0; ++use; }
     };
-    for (int i = 0; i < n_tiles + 2 && ok; ++i) {
-      if (i >= 2) {  // O += P[j] V[j]; P[j] lies over S[j]: 16 keys = 8 columns of bf16 pairs
-        const int j = i - 2;
-        if (!(ok = mbar_wait_warp(bar_p + 8 * (j & 1), (uint32_t)((j >> 1) & 1), abort_flag))) break;
-        tc_fence_after();
-        const int valid = keys.valid(j, p, tile);
-        constexpr uint32_t idesc = umma_idesc(128, HD, 1);
-        const uint32_t pj = tmem + S_COL + (j & 1) * KT;
-        for (int s = 0; s * KSUB < valid && wait_slot(); ++s) {
-          const int left = valid - s * KSUB;
-          const uint64_t dv = umma_desc(ring + slot * SLOT, KSUB * 128, 1024);
-          if (left >= KSUB) {
-            if (el) {
+    for (int k = 0; k < n_items && ok; ++k) {
+      const Item it(p, table, k, total);
+      const Keys keys(p, it.tile, it.z, p.parts);
+      if (keys.n == 0) continue;
+      if (!(ok = mbar_wait_warp(bar_q, (uint32_t)live & 1, abort_flag))) break;
+      uint32_t early_p = 0;
+      for (int i = 0; i < keys.n + 2 && ok; ++i) {
+        if (i >= 2) {  // O += P[j] V[j]; P[j] lies over S[j]: 16 keys = 8 columns of bf16 pairs
+          const int j = i - 2, J = jj + j;
+          if (!(ok = __all_sync(0xffffffffu, early_p != 0) || mbar_wait_warp(bar_p + 8 * (J & 1), (uint32_t)(J >> 1) & 1, abort_flag))) break;
+          if (j == 0 && live > 0 && !(ok = mbar_wait_warp(bar_o_free, (uint32_t)(live - 1) & 1, abort_flag))) break;  // O of the item before has been read
+          tc_fence_after();
+          const int valid = keys.valid(j, p, it.tile);
+          constexpr uint32_t idesc = umma_idesc(128, HD, 1);
+          const uint32_t pj = tmem + S_COL + (J & 1) * KT;
+          for (int s = 0; s < VP && wait_slot(); ++s) {
+            const int left = valid - s * KSUB;
+            const uint64_t dv = umma_desc(ring + slot * SLOT, KSUB * 128, 1024);
+            if (left >= KSUB) {
+              ask_next();
+              if (el) {
 #pragma unroll
-              for (int k = 0; k < KSUB / 16; ++k) umma_f16_ts(tmem, pj + (s * (KSUB / 16) + k) * 8, dv + (uint64_t)(k * 128), idesc, (j | s | k) != 0 ? 1u : 0u);
-              umma_commit_to(empty + 8 * slot);
-            }
-          } else {
-            const int steps = (left + 15) >> 4;
-            if (left & 15) {  // rows behind the last key of the step
-              const int rows = steps * 16 - left;
-              for (int z = lane; z < rows * NKB * 8; z += 32) {
-                const int r = z / (NKB * 8), c = z - r * (NKB * 8);
-                *reinterpret_cast<uint4*>(smem + D::Q_BYTES + slot * SLOT + (c >> 3) * (KSUB * 128) + (left + r) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                for (int x = 0; x < KSUB / 16; ++x) umma_f16_ts(tmem, pj + (s * (KSUB / 16) + x) * 8, dv + (uint64_t)(x * 128), idesc, (j | s | x) != 0 ? 1u : 0u);
+                umma_commit_to(empty + 8 * slot);
               }
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              __syncwarp();
+            } else {
+              const int steps = max(0, (left + 15) >> 4);
+              if (left > 0 && (left & 15)) {  // rows behind the last key of the step
+                const int rows = steps * 16 - left;
+                for (int z = lane; z < rows * NKB * 8; z += 32) {
+                  const int r = z / (NKB * 8), c = z - r * (NKB * 8);
+                  *reinterpret_cast<uint4*>(smem + D::Q_BYTES + slot * SLOT + (c >> 3) * (KSUB * 128) + (left + r) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+              }
+              ask_next();
+              if (el) {
+                for (int x = 0; x < steps; ++x) umma_f16_ts(tmem, pj + (s * (KSUB / 16) + x) * 8, dv + (uint64_t)(x * 128), idesc, (j | s | x) != 0 ? 1u : 0u);
+                umma_commit_to(empty + 8 * slot);
+              }
             }
+            advance();
+          }
+          if (!ok) break;
+          if (el) {
+            umma_commit_to(bar_o + 8 * (J & 1));
+            if (j + 1 == keys.n) umma_commit_to(bar_done);
+          }
+        }
+        early_p = 0;
+        if (i < keys.n) {  // S[i]
+          const int J = jj + i;
+          const int valid = keys.valid(i, p, it.tile);
+          const uint32_t d = tmem + S_COL + (J & 1) * KT;
+          // a partial tile: the columns that hold a key, rounded up to the instruction's 16
+          const uint32_t idesc = valid == KT ? umma_idesc(128, KT, 0) : umma_idesc(128, 0, 0) | ((uint32_t)((valid + 15) >> 4) << 18);
+          for (int s = 0; s < KP && wait_slot(); ++s) {
+            ask_next();
             if (el) {
-              for (int k = 0; k < steps; ++k) umma_f16_ts(tmem, pj + (s * (KSUB / 16) + k) * 8, dv + (uint64_t)(k * 128), idesc, (j | s | k) != 0 ? 1u : 0u);
+#pragma unroll
+              for (int c = 0; c < SLABS; ++c) {
+                const uint64_t dq = umma_desc(q_base + (s * SLABS + c) * 16384, 16, 1024), dk = umma_desc(ring + slot * SLOT + c * 16384, 16, 1024);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) umma_f16(d, dq + (uint64_t)(x * 2), dk + (uint64_t)(x * 2), idesc, (s | c | x) != 0 ? 1u : 0u);
+              }
               umma_commit_to(empty + 8 * slot);
             }
+            if (i >= 1 && s + 1 == KP) early_p = mbar_test(bar_p + 8 * ((J - 1) & 1), (uint32_t)((J - 1) >> 1) & 1);
+            advance();
           }
-          advance();
-        }
-        if (!ok) break;
-        if (el) {
-          umma_commit_to(bar_o + 8 * (j & 1));
-          if (j + 1 == n_tiles) umma_commit_to(bar_done);
+          if (ok && el) {
+            umma_commit_to(bar_s + 8 * (J & 1));
+            if (i + 1 == keys.n) umma_commit_to(bar_q_free);
+          }
         }
       }
-      if (i < n_tiles) {  // S[i]
-        const int valid = keys.valid(i, p, tile);
-        const uint32_t d = tmem + S_COL + (i & 1) * KT;
-        // a partial tile: the columns that hold a key, rounded up to the instruction's 16
-        const uint32_t idesc = valid == KT ? umma_idesc(128, KT, 0) : umma_idesc(128, 0, 0) | ((uint32_t)((valid + 15) >> 4) << 18);
-        for (int s = 0; s < NKB / SLABS && wait_slot(); ++s) {
-          if (el) {
-#pragma unroll
-            for (int c = 0; c < SLABS; ++c) {
-              const uint64_t dq = umma_desc(q_base + (s * SLABS + c) * 16384, 16, 1024), dk = umma_desc(ring + slot * SLOT + c * 16384, 16, 1024);
-#pragma unroll
-              for (int k = 0; k < 4; ++k) umma_f16(d, dq + (uint64_t)(k * 2), dk + (uint64_t)(k * 2), idesc, (s | c | k) != 0 ? 1u : 0u);
-            }
-            umma_commit_to(empty + 8 * slot);
-          }
-          advance();
-        }
-        if (ok && el) umma_commit_to(bar_s + 8 * (i & 1));
-      }
+      advance();  // the epilogue's slot
+      early = 0;
+      jj += keys.n;
+      ++live;
     }
   } else {
     // ---- softmax: group h takes the tiles of its parity; thread r of a group has row r ----------------------------------------------
     const int h = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_tmem = tmem + lanes + S_COL + h * KT;
-    const int tok = tile.t0 + r / G;  // the row's token in its question
-    float m = -INFINITY, l = 0.f;     // what this group's part of the denominator is relative to, and that part
+    const int tt = r / G;  // the row's token in the tile
     bool ok = true;
-    for (int j = h; j < n_tiles && ok; j += 2) {
-      const uint32_t ph = (uint32_t)((j >> 1) & 1);
+    int live = 0, jj = 0;
+    uint32_t slots_used = 0;
+    for (int k = 0; k < n_items && ok; ++k) {
+    const Item it(p, table, k, total);
+    const Tile& tile = it.tile;
+    const Keys keys(p, tile, it.z, p.parts);
+    const int n_tiles = keys.n;
+    const size_t block_lin = ((size_t)it.z * nh + it.hg) * p.max_tiles + it.ti;
+    if (n_tiles == 0) {  // more parts than key tiles
+      if (h == 0) p.ws_ml[block_lin * 128 + r] = make_float2(-INFINITY, 0.f);
+      continue;
+    }
+    const int tok = tile.t0 + tt;  // ... and in its question
+    if (p.gate_qg && p.parts == 1 && tt < tile.ntok) {  // the item's gates come to L2 now: all CTAs reach their epilogues at about the same time
+      const bf16* gate = p.gate_qg + ((size_t)tile.off + tok) * p.qg_stride + (size_t)(2 * (it.head0 + r - tt * G) + 1) * HD + h * (HD / 2);
+#pragma unroll
+      for (int i = 0; i < HD / 2; i += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(gate + i));
+    }
+    float m = -INFINITY, l = 0.f;  // what this group's part of the denominator is relative to, and that part
+    for (int j = (h ^ jj) & 1; j < n_tiles && ok; j += 2) {
+      const uint32_t ph = (uint32_t)((jj + j) >> 1) & 1, ph_before = (uint32_t)((jj + j - 1) >> 1) & 1;
       int lim = keys.valid(j, p, tile);
       if (p.causal && !keys.state(j)) lim = min(lim, tok + 1 - keys.key0(j));
-      ok = __all_sync(0xffffffffu, mbar_wait(bar_s + 8 * h, ph, abort_flag));
-      if (!ok) break;
-      tc_fence_after();
-      float x[KT];
-#pragma unroll
-      for (int i = 0; i < KT; i += 32) tmem_ld32(s_tmem + i, reinterpret_cast<uint32_t*>(x + i));
-      tmem_ld_wait();
-      if (__any_sync(0xffffffffu, lim < KT)) {
-#pragma unroll
-        for (int i = 0; i < KT; ++i) x[i] = i < lim ? x[i] : -INFINITY;
-      }
-      float t4[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-      for (int i = 4; i < KT; ++i) t4[i & 3] = fmaxf(t4[i & 3], x[i]);
-      const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * p.scale_log2e;
-      // the maximum in use so far, from the other group's tile before this one
+      // the maximum in use so far, from the other group's tile before this one: published long before S[j] is there
       float before = -INFINITY;
       if (j > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_m + 8 * (h ^ 1), (uint32_t)(((j - 1) >> 1) & 1), abort_flag));
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_m + 8 * (h ^ 1), ph_before, abort_flag));
         if (!ok) break;
         before = m_used[(h ^ 1) * 128 + r];
       }
+      ok = __all_sync(0xffffffffu, mbar_wait(bar_s + 8 * h, ph, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      // The scores are read from TMEM twice, 64 at a time, once for the maximum and once for the weights: a thread that keeps all 128 has
+      // none of its registers left, and the straight code for them evicts the issuing warp's from the instruction cache (419 -> 364 us
+      // over 64 questions of about 107 tokens and 2048 keys).
+      const bool partial = __any_sync(0xffffffffu, lim < KT);
+      float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+      for (int c = 0; c < KT; c += 64) {
+        float x[64];
+#pragma unroll
+        for (int i = 0; i < 64; i += 32) tmem_ld32(s_tmem + c + i, reinterpret_cast<uint32_t*>(x + i));
+        tmem_ld_wait();
+        if (partial) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) x[i] = c + i < lim ? x[i] : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 64; ++i) t4[i & 3] = fmaxf(t4[i & 3], x[i]);
+      }
+      const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * p.scale_log2e;
       const float now = top > before + RESCALE ? top : before;
       m_used[h * 128 + r] = now;
       mbar_arrive(bar_m + 8 * h);
       if (j > 0 && __any_sync(0xffffffffu, now != before)) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_o + 8 * (h ^ 1), (uint32_t)(((j - 1) >> 1) & 1), abort_flag));  // O is at rest
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_o + 8 * (h ^ 1), ph_before, abort_flag));  // O is at rest
         if (!ok) break;
         tc_fence_after();
         const float f = now != before ? ex2(before - now) : 1.0f;
@@ -408,87 +537,123 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
       const float neg = now == -INFINITY ? 0.f : -now;  // a row that has seen nothing: every weight 2^-inf
       float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int c = 0; c < KT; c += 64) {
+        float x[64];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+        for (int i = 0; i < 64; i += 32) tmem_ld32(s_tmem + c + i, reinterpret_cast<uint32_t*>(x + i));
+        tmem_ld_wait();
+        if (partial) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) x[i] = c + i < lim ? x[i] : -INFINITY;
+        }
         uint32_t w[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          const float a = ex2(fmaf(x[half * 64 + 2 * i], p.scale_log2e, neg)), b = ex2(fmaf(x[half * 64 + 2 * i + 1], p.scale_log2e, neg));
+          const float a = ex2(fmaf(x[2 * i], p.scale_log2e, neg)), b = ex2(fmaf(x[2 * i + 1], p.scale_log2e, neg));
           l4[(2 * i) & 3] += a;
           l4[(2 * i + 1) & 3] += b;
           w[i] = pack_bf16(a, b);
         }
-        tmem_st32(s_tmem + half * 32, w);
+        tmem_st32(s_tmem + c / 2, w);
       }
       l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(bar_p + 8 * h);
     }
-    // ---- epilogue: either group takes half of the head's dimensions --------------------------------------------------------------
-    const int last = (n_tiles - 1) & 1, tt = r / G, head = head0 + r - tt * G;
-    const bool live = tt < tile.ntok;
-    const size_t t = (size_t)tile.off + tile.t0 + tt;
-    const bf16* gate = p.gate_qg && live && gridDim.z == 1 ? p.gate_qg + t * p.qg_stride + (size_t)(2 * head + 1) * HD + h * (HD / 2) : nullptr;
-    uint4 gv[HD / 16];  // on their way while the last product runs
-    if (gate) {
+    // ---- epilogue: either group takes half of the head's dimensions, each warp its 32 rows, CH dimensions at a time: from TMEM (lane =
+    // row) to the warp's part of the epilogue's slot, and from there in whole rows ---------------------------------------------------
+    constexpr int CH = SLOT / 1024, LPR = CH / 4, RPP = 32 / LPR, PASSES = 32 / RPP;  // lanes per row, rows per pass
+    const int last_j = jj + n_tiles - 1, last = last_j & 1;
+    slots_used += (uint32_t)n_tiles * (KP + VP);
+    const int e_slot = (int)(slots_used % SLOTS);
+    const uint32_t e_phase = (slots_used / SLOTS) & 1;
+    ++slots_used;
+    // a lane's rows, four dimensions of each: where they go, and the gates of the first dimensions, on their way under the last product
+    const int my_row = lane / LPR, my_c = lane % LPR;
+    const float inv_g = 1.0f / (float)G;
+    const bf16* gate0 = p.parts == 1 && p.gate_qg ? p.gate_qg + ((size_t)tile.off + tile.t0) * p.qg_stride + (size_t)(2 * it.head0 + 1) * HD + h * (HD / 2) + my_c * 4 : nullptr;
+    bf16* out0 = p.out + (((size_t)tile.off + tile.t0) * p.heads + it.head0) * HD + h * (HD / 2) + my_c * 4;
+    uint32_t gate_at[PASSES], out_at[PASSES];  // offsets of the rows; ~0: not a row of the question
 #pragma unroll
-      for (int i = 0; i < HD / 16; ++i) gv[i] = *reinterpret_cast<const uint4*>(gate + i * 8);
+    for (int ps = 0; ps < PASSES; ++ps) {
+      const int R = (warp & 3) * 32 + ps * RPP + my_row, rt = (int)(((float)R + 0.5f) * inv_g);  // R / G, exact below 128
+      const bool there = rt < tile.ntok;
+      gate_at[ps] = (uint32_t)rt * (uint32_t)p.qg_stride + (uint32_t)(2 * (R - rt * G)) * HD;
+      out_at[ps] = there ? (uint32_t)(rt * p.heads + R - rt * G) * HD : ~0u;
     }
-    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar_m + 8 * last, (uint32_t)(((n_tiles - 1) >> 1) & 1), abort_flag));
+    uint2 gv[PASSES];
+    auto load_gates = [&](int c) {
+#pragma unroll
+      for (int ps = 0; ps < PASSES; ++ps)
+        gv[ps] = ld_global_if(gate0 + gate_at[ps] + c, out_at[ps] != ~0u);
+    };
+    if (gate0) load_gates(0);
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar_m + 8 * last, (uint32_t)(last_j >> 1) & 1, abort_flag));
     float end_m = -INFINITY;
     if (ok) {
       end_m = m_used[last * 128 + r];
-      ok = __all_sync(0xffffffffu, mbar_wait(bar_done, 0, abort_flag));
-    }
-    if (ok) {
       l_part[h * 128 + r] = m == -INFINITY ? 0.f : l * ex2(m - end_m);
       mbar_arrive(bar_l);
-      ok = __all_sync(0xffffffffu, mbar_wait(bar_l, 0, abort_flag));
+      ok = __all_sync(0xffffffffu, mbar_wait(bar_l, (uint32_t)live & 1, abort_flag));
     }
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar_done, (uint32_t)live & 1, abort_flag));
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * e_slot, e_phase, abort_flag));
     if (ok) {
       tc_fence_after();
       const float sum = l_part[r] + l_part[128 + r];
-      if (gridDim.z > 1) {
-        if (h == 0) p.ws_ml[block_lin * 128 + r] = make_float2(end_m, sum);
-        float* dst = p.ws_o + (block_lin * 128 + r) * HD;
+      if (p.parts > 1 && h == 0) p.ws_ml[block_lin * 128 + r] = make_float2(end_m, sum);
+      const float inv = p.parts > 1 ? 1.0f : sum > 0.f ? 1.0f / sum : 0.f;
+      uint8_t* stage = smem + D::Q_BYTES + e_slot * SLOT + warp * (SLOT / 8);
+      auto swz = [](int row) { return CH == 32 ? row & 7 : (row >> 1) & 3; };  // 16-byte chunks of a row: no two lanes of a quarter in one bank
 #pragma unroll 1
-        for (int c = h * (HD / 2); c < (h + 1) * (HD / 2); c += 32) {
-          uint32_t v[32];
-          tmem_ld32(tmem + lanes + c, v);
-          tmem_ld_wait();
-          if (live) {
+      for (int c = 0; c < HD / 2; c += CH) {
+        uint32_t v[CH];
+        if constexpr (CH == 32) tmem_ld32(tmem + lanes + h * (HD / 2) + c, v);
+        else tmem_ld16(tmem + lanes + h * (HD / 2) + c, v);
+        tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-          }
+        for (int i = 0; i < LPR; ++i)
+          *reinterpret_cast<float4*>(stage + lane * (CH * 4) + ((i ^ swz(lane)) * 16)) =
+              make_float4(__uint_as_float(v[4 * i]) * inv, __uint_as_float(v[4 * i + 1]) * inv, __uint_as_float(v[4 * i + 2]) * inv, __uint_as_float(v[4 * i + 3]) * inv);
+        __syncwarp();
+        float4 o[PASSES];
+#pragma unroll
+        for (int ps = 0; ps < PASSES; ++ps) {
+          const int row = ps * RPP + my_row;
+          o[ps] = *reinterpret_cast<const float4*>(stage + row * (CH * 4) + ((my_c ^ swz(row)) * 16));
         }
-      } else {
-        const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-        bf16* dst = p.out + (t * p.heads + head) * HD + h * (HD / 2);
+        if (p.parts > 1) {
 #pragma unroll
-        for (int c = 0; c < HD / 2; c += 32) {
-          uint32_t v[32];
-          tmem_ld32(tmem + lanes + h * (HD / 2) + c, v);
-          tmem_ld_wait();
-          if (live) {
+          for (int ps = 0; ps < PASSES; ++ps)
+            if (out_at[ps] != ~0u)
+              *reinterpret_cast<float4*>(p.ws_o + (block_lin * 128 + (warp & 3) * 32 + ps * RPP + my_row) * HD + h * (HD / 2) + c + my_c * 4) = o[ps];
+        } else {
+          if (gate0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float o[8];
-#pragma unroll
-              for (int k = 0; k < 8; ++k) o[k] = __uint_as_float(v[i * 8 + k]) * inv;
-              if (gate) {
-                const __nv_bfloat162* g2 = reinterpret_cast<const __nv_bfloat162*>(&gv[c / 8 + i]);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  o[2 * k] *= __fdividef(1.0f, 1.0f + __expf(-__low2float(g2[k])));
-                  o[2 * k + 1] *= __fdividef(1.0f, 1.0f + __expf(-__high2float(g2[k])));
-                }
-              }
-              *reinterpret_cast<uint4*>(dst + c + i * 8) = make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7]));
+            for (int ps = 0; ps < PASSES; ++ps) {
+              const __nv_bfloat162* g2 = reinterpret_cast<const __nv_bfloat162*>(&gv[ps]);
+              o[ps].x *= gate_of(__low2float(g2[0]));
+              o[ps].y *= gate_of(__high2float(g2[0]));
+              o[ps].z *= gate_of(__low2float(g2[1]));
+              o[ps].w *= gate_of(__high2float(g2[1]));
             }
+            if (c + CH < HD / 2) load_gates(c + CH);
           }
+#pragma unroll
+          for (int ps = 0; ps < PASSES; ++ps)
+            st_global_if(out0 + out_at[ps] + c, make_uint2(pack_bf16(o[ps].x, o[ps].y), pack_bf16(o[ps].z, o[ps].w)), out_at[ps] != ~0u);
         }
+        __syncwarp();
       }
+      tc_fence_before();
+      mbar_arrive(bar_o_free);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the slot goes back to TMA
+      mbar_arrive(bar_e);
+    }
+    jj += n_tiles;
+    ++live;
     }
   }
 
@@ -510,11 +675,21 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 template <int HD>
 __global__ void __launch_bounds__(128) kv4_attention_merge_kernel(const Params p, int parts) {
   constexpr int PER = HD / 32;
-  __shared__ int sums[8];
-  Tile tile;
-  if (!find_tile(p, blockIdx.x, p.causal != 0, sums, tile)) return;
+  __shared__ int sums[4], found[3];
+  if (threadIdx.x == 0) found[0] = -1;
+  __syncthreads();
+  scan_tiles(p, sums, [&](int b, int before, int n) {
+    const int ti = blockIdx.x;
+    if (ti < before || ti >= before + n) return;
+    int off, len;
+    tiles_of(p, b, off, len);
+    found[0] = off;
+    found[1] = (ti - before) * p.tokens;
+    found[2] = min(p.tokens, len - found[1]);
+  });
+  __syncthreads();
   const int lane = threadIdx.x & 31, r = blockIdx.z * 4 + (threadIdx.x >> 5), G = p.G;
-  if (r >= tile.ntok * G) return;
+  if (found[0] < 0 || r >= found[2] * G) return;
   const int hg = blockIdx.y, kh = hg / p.sub, tt = r / G;
   const int head = kh * (p.heads / p.kv) + (hg - kh * p.sub) * G + r - tt * G;
   const size_t step = (size_t)gridDim.y * gridDim.x * 128, row0 = ((size_t)hg * gridDim.x + blockIdx.x) * 128 + r;
@@ -541,7 +716,7 @@ __global__ void __launch_bounds__(128) kv4_attention_merge_kernel(const Params p
       acc[i + 1] += w * v.y;
     }
   }
-  const size_t t = (size_t)tile.off + tile.t0 + tt;
+  const size_t t = (size_t)found[0] + found[1] + tt;
   const float inv = sum > 0.f ? 1.0f / sum : 0.f;
   const bf16* gate = p.gate_qg ? p.gate_qg + t * p.qg_stride + (size_t)(2 * head + 1) * HD + lane * PER : nullptr;
   bf16* dst = p.out + (t * p.heads + head) * HD + lane * PER;
@@ -607,6 +782,8 @@ cudaError_t run(const Kv4QuestionArgs& a, const Plan& pl, uint8_t* ws, cudaStrea
   p.out = a.out;
   p.scale_log2e = (1.0f / sqrtf((float)HD)) * 1.4426950408889634f;
   p.err = a.err;
+  p.parts = pl.parts;
+  p.max_tiles = pl.tiles;
   p.ws_ml = (float2*)(ws + pl.state_bytes);
   p.ws_o = (float*)(ws + pl.state_bytes + pl.ml_bytes);
   const uint64_t width = (uint64_t)a.kv * HD;
@@ -625,7 +802,10 @@ cudaError_t run(const Kv4QuestionArgs& a, const Plan& pl, uint8_t* ws, cudaStrea
   if (bad) return cudaErrorInvalidValue;
   if (a.n_state > 0) CUDA_TRY(launch_kv4_read<bf16>(a.state, a.n_state, nullptr, ks, vs, a.n_state, a.kv, HD, nullptr, s));
   CUDA_TRY(cudaFuncSetAttribute(kv4_attention_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<HD>::SMEM));
-  const dim3 grid(pl.tiles, a.kv * pl.sub, pl.parts);
+  // one CTA per SM, more only where one would have more items than its table holds
+  const long long items = (long long)pl.tiles * a.kv * pl.sub * pl.parts;
+  if (items > (1 << 30)) return cudaErrorInvalidValue;
+  const unsigned grid = (unsigned)max(min(items, (long long)sm_count()), (items + MAX_ITEMS - 1) / MAX_ITEMS);
   auto map = [](const TcTensorMap& m) -> const CUtensorMap& { return *reinterpret_cast<const CUtensorMap*>(&m); };
   kv4_attention_kernel<HD><<<grid, NUM_THREADS, Shape<HD>::SMEM, s>>>(map(q), map(ksm), map(vsm), map(ko), map(vo), p);
   CUDA_TRY(cudaGetLastError());
