@@ -6,7 +6,9 @@
 // exact in bf16, and attention over the cache is attention over exactly those bf16 values.
 //
 // Both kernels move each byte once and do a few operations a value: bound by HBM (write: 2 bytes a bf16 value in, 0.5625 out). One
-// thread handles one group of 16, so that a warp's loads, its code words and its scale bytes are each contiguous.
+// thread handles one group of 16 of K and the same one of V, so that a warp's code words and scale bytes are contiguous and a thread has
+// both of its loads in flight; the 32 bytes of a bf16 group go in one 256-bit access (as two of 16 bytes each store would touch 32
+// sectors by half).
 #include "common.cuh"
 #include "kv4.h"
 
@@ -25,28 +27,40 @@ __device__ __forceinline__ uint32_t e2m1_code(float x) {
   return m | (x < 0.f ? 8u : 0u);
 }
 
-template <typename T, bool WIDE>
+__device__ __forceinline__ void ld256(const void* p, uint32_t (&u)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void st256(void* p, const uint32_t (&u)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]),
+               "r"(u[7])
+               : "memory");
+}
+
+// 16 consecutive values. ALIGN: 32-byte accesses, 16-byte ones, or one value at a time.
+template <typename T, int ALIGN>
 __device__ __forceinline__ void load16(const T* p, float (&f)[16]) {
-  if constexpr (WIDE && sizeof(T) == 2) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint4 u = reinterpret_cast<const uint4*>(p)[h];
-      const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&u);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f[8 * h + 2 * i] = __low2float(b[i]);
-        f[8 * h + 2 * i + 1] = __high2float(b[i]);
-      }
-    }
-  } else if constexpr (WIDE) {
-#pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      const float4 u = reinterpret_cast<const float4*>(p)[h];
-      f[4 * h] = u.x; f[4 * h + 1] = u.y; f[4 * h + 2] = u.z; f[4 * h + 3] = u.w;
-    }
-  } else {
+  if constexpr (ALIGN == 1) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) f[i] = Ty<T>::ld(p + i);
+  } else {
+    constexpr int WORDS = 4 * (int)sizeof(T);
+    uint32_t u[WORDS];
+#pragma unroll
+    for (int h = 0; h < WORDS; h += 8) {
+      uint32_t q[8];
+      if constexpr (ALIGN == 32) {
+        ld256(reinterpret_cast<const uint32_t*>(p) + h, q);
+      } else {
+        const uint4 a = reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + h)[0], b = reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + h)[1];
+        q[0] = a.x; q[1] = a.y; q[2] = a.z; q[3] = a.w; q[4] = b.x; q[5] = b.y; q[6] = b.z; q[7] = b.w;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u[h + i] = q[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) f[i] = sizeof(T) == 4 ? __uint_as_float(u[i < WORDS ? i : 0]) : __uint_as_float(i & 1 ? u[i >> 1] & 0xffff0000u : u[i >> 1] << 16);
   }
 }
 
@@ -68,74 +82,85 @@ __device__ __forceinline__ void encode16(const float (&f)[16], uint2& codes, uin
   }
 }
 
-// blockIdx.y: 0 K, 1 V
-template <typename T, bool WIDE>
-__global__ void __launch_bounds__(256) kv4_write_kernel(const T* __restrict__ k, size_t k_stride, const T* __restrict__ v, size_t v_stride,
-                                                        const int64_t* __restrict__ slots, uint8_t* __restrict__ k_codes, uint8_t* __restrict__ k_scales,
-                                                        uint8_t* __restrict__ v_codes, uint8_t* __restrict__ v_scales, size_t cache_rows, size_t rows,
-                                                        int groups, int* err) {
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * groups) return;
-  const size_t row = i / (uint32_t)groups;
-  const uint32_t j = (uint32_t)(i - row * groups);
+// The cache row of token `row`, or -1: it is left out. I: an index type that holds rows * groups (divisions by the group count are
+// most of what a thread computes beside its conversions).
+__device__ __forceinline__ int64_t cache_row(const int64_t* slots, size_t row, size_t cache_rows, int* err) {
   const int64_t slot = slots ? slots[row] : (int64_t)row;
-  if (slot < 0) return;
-  if ((uint64_t)slot >= cache_rows) {
+  if (slot >= 0 && (uint64_t)slot >= cache_rows) {
     set_err(err, DERR_CACHE_ROW);
-    return;
+    return -1;
   }
-  const bool second = blockIdx.y != 0;
-  const T* src = (second ? v + row * v_stride : k + row * k_stride) + (size_t)j * 16;
-  float f[16];
-  load16<T, WIDE>(src, f);
-  uint2 codes;
-  uint8_t scale;
-  encode16<T>(f, codes, scale);
-  const size_t at = (size_t)slot * groups + j;
-  reinterpret_cast<uint2*>(second ? v_codes : k_codes)[at] = codes;
-  (second ? v_scales : k_scales)[at] = scale;
+  return slot < 0 ? -1 : slot;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Cache c, size_t cache_rows, const int64_t* __restrict__ slots, T* __restrict__ k,
-                                                       T* __restrict__ v, size_t rows, int groups, int* err) {
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * groups) return;
-  const size_t row = i / (uint32_t)groups;
+template <typename T, int ALIGN, typename I>
+__global__ void __launch_bounds__(256) kv4_write_kernel(const T* __restrict__ k, size_t k_stride, const T* __restrict__ v, size_t v_stride,
+                                                        const int64_t* __restrict__ slots, uint8_t* __restrict__ k_codes, uint8_t* __restrict__ k_scales,
+                                                        uint8_t* __restrict__ v_codes, uint8_t* __restrict__ v_scales, size_t cache_rows, I total,
+                                                        uint32_t groups, int* err) {
+  const I i = (I)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const I row = i / groups;
   const uint32_t j = (uint32_t)(i - row * groups);
-  const int64_t slot = slots ? slots[row] : (int64_t)row;
+  const int64_t slot = cache_row(slots, row, cache_rows, err);
   if (slot < 0) return;
-  if ((uint64_t)slot >= cache_rows) {
-    set_err(err, DERR_CACHE_ROW);
-    return;
-  }
-  const Kv4Part part = blockIdx.y ? c.v : c.k;
+  float fk[16], fv[16];
+  load16<T, ALIGN>(k + row * k_stride + (size_t)j * 16, fk);
+  load16<T, ALIGN>(v + row * v_stride + (size_t)j * 16, fv);
   const size_t at = (size_t)slot * groups + j;
-  const uint2 w = reinterpret_cast<const uint2*>(part.codes)[at];
-  const __half_raw hr = __nv_cvt_fp8_to_halfraw(part.scales[at], __NV_E4M3);
+  uint2 codes;
+  uint8_t scale;
+  encode16<T>(fk, codes, scale);
+  reinterpret_cast<uint2*>(k_codes)[at] = codes;
+  k_scales[at] = scale;
+  encode16<T>(fv, codes, scale);
+  reinterpret_cast<uint2*>(v_codes)[at] = codes;
+  v_scales[at] = scale;
+}
+
+// e2m1 * e4m3 is exact in f16, and in either output type
+template <typename T>
+__device__ __forceinline__ void decode16(const uint2 w, uint8_t scale, T* dst) {
+  const __half_raw hr = __nv_cvt_fp8_to_halfraw(scale, __NV_E4M3);
   const __half2 s2 = __half2half2(*reinterpret_cast<const __half*>(&hr));
-  T* dst = (blockIdx.y ? v : k) + i * 16;
-  float f[16];
+  uint32_t u[4 * sizeof(T)];
 #pragma unroll
-  for (int b = 0; b < 8; ++b) {  // e2m1 * e4m3 is exact in f16, and in either output type
+  for (int b = 0; b < 8; ++b) {
     const __half2_raw pr = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)((b < 4 ? w.x : w.y) >> (8 * (b & 3))), __NV_E2M1);
     const float2 p = __half22float2(__hmul2(*reinterpret_cast<const __half2*>(&pr), s2));
-    f[2 * b] = p.x;
-    f[2 * b + 1] = p.y;
-  }
-  if constexpr (sizeof(T) == 2) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint4 u;
-      __nv_bfloat162* b2 = reinterpret_cast<__nv_bfloat162*>(&u);
-#pragma unroll
-      for (int n = 0; n < 4; ++n) b2[n] = __floats2bfloat162_rn(f[8 * h + 2 * n], f[8 * h + 2 * n + 1]);
-      reinterpret_cast<uint4*>(dst)[h] = u;
+    if constexpr (sizeof(T) == 2) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(p.x, p.y);
+      u[b] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      u[2 * b] = __float_as_uint(p.x);
+      u[2 * b + 1] = __float_as_uint(p.y);
     }
-  } else {
-#pragma unroll
-    for (int h = 0; h < 4; ++h) reinterpret_cast<float4*>(dst)[h] = make_float4(f[4 * h], f[4 * h + 1], f[4 * h + 2], f[4 * h + 3]);
   }
+#pragma unroll
+  for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
+    uint32_t q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = u[8 * h + i];
+    st256(reinterpret_cast<uint32_t*>(dst) + 8 * h, q);
+  }
+}
+
+template <typename T, typename I>
+__global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Cache c, size_t cache_rows, const int64_t* __restrict__ slots, T* __restrict__ k,
+                                                       T* __restrict__ v, I total, uint32_t groups, int* err) {
+  const I i = (I)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  size_t at = i;
+  if (slots) {
+    const I row = i / groups;
+    const int64_t slot = cache_row(slots, row, cache_rows, err);
+    if (slot < 0) return;
+    at = (size_t)slot * groups + (size_t)(i - row * groups);
+  }
+  const uint2 wk = reinterpret_cast<const uint2*>(c.k.codes)[at], wv = reinterpret_cast<const uint2*>(c.v.codes)[at];
+  const uint8_t sk = c.k.scales[at], sv = c.v.scales[at];
+  decode16<T>(wk, sk, k + (size_t)i * 16);
+  decode16<T>(wv, sv, v + (size_t)i * 16);
 }
 
 }  // namespace
@@ -144,20 +169,31 @@ template <typename T>
 cudaError_t launch_kv4_write(const T* k, size_t k_stride, const T* v, size_t v_stride, const int64_t* slots, uint8_t* k_codes, uint8_t* k_scales,
                              uint8_t* v_codes, uint8_t* v_scales, size_t cache_rows, int rows, int kv, int hd, int* err, cudaStream_t s) {
   if (rows <= 0) return cudaSuccess;
-  constexpr int V = 16 / (int)sizeof(T);
-  const int groups = kv * (hd / 16);
-  const dim3 grid((unsigned)(((size_t)rows * groups + 255) / 256), 2);
-  const bool wide = k_stride % V == 0 && v_stride % V == 0 && reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0;
-  (wide ? kv4_write_kernel<T, true> : kv4_write_kernel<T, false>)<<<grid, 256, 0, s>>>(k, k_stride, v, v_stride, slots, k_codes, k_scales, v_codes, v_scales,
-                                                                                       cache_rows, (size_t)rows, groups, err);
+  const uint32_t groups = (uint32_t)kv * (hd / 16);
+  const size_t total = (size_t)rows * groups;
+  const unsigned grid = (unsigned)((total + 255) / 256);
+  auto at_steps = [&](size_t bytes) {  // rows and pointers on multiples of so many bytes
+    return k_stride * sizeof(T) % bytes == 0 && v_stride * sizeof(T) % bytes == 0 && (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % bytes == 0;
+  };
+#define KV4_WRITE(ALIGN, I) \
+  kv4_write_kernel<T, ALIGN, I><<<grid, 256, 0, s>>>(k, k_stride, v, v_stride, slots, k_codes, k_scales, v_codes, v_scales, cache_rows, (I)total, groups, err)
+  if (total >= (1u << 31)) {
+    if (at_steps(16)) KV4_WRITE(16, size_t);
+    else KV4_WRITE(1, size_t);
+  } else if (at_steps(32)) KV4_WRITE(32, uint32_t);
+  else if (at_steps(16)) KV4_WRITE(16, uint32_t);
+  else KV4_WRITE(1, uint32_t);
+#undef KV4_WRITE
   return cudaGetLastError();
 }
 template <typename T>
 cudaError_t launch_kv4_read(const Kv4Cache& c, size_t cache_rows, const int64_t* slots, T* k, T* v, int rows, int kv, int hd, int* err, cudaStream_t s) {
   if (rows <= 0) return cudaSuccess;
-  const int groups = kv * (hd / 16);
-  const dim3 grid((unsigned)(((size_t)rows * groups + 255) / 256), 2);
-  kv4_read_kernel<T><<<grid, 256, 0, s>>>(c, cache_rows, slots, k, v, (size_t)rows, groups, err);
+  const uint32_t groups = (uint32_t)kv * (hd / 16);
+  const size_t total = (size_t)rows * groups;
+  const unsigned grid = (unsigned)((total + 255) / 256);
+  if (total >= (1u << 31)) kv4_read_kernel<T, size_t><<<grid, 256, 0, s>>>(c, cache_rows, slots, k, v, total, groups, err);
+  else kv4_read_kernel<T, uint32_t><<<grid, 256, 0, s>>>(c, cache_rows, slots, k, v, (uint32_t)total, groups, err);
   return cudaGetLastError();
 }
 #define INST_KV4(T)                                                                                                                                     \
