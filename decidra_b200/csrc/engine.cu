@@ -355,7 +355,8 @@ int gemm(dcd_engine* e, const void* X, const TcTensorMap* tmA, const void* W, co
     return DCD_OK;
   }
   if (act_out) return fail(e, DCD_E_INVALID, "internal: fused SwiGLU quantisation on a GEMM that does not take the block-scaled path");
-  if (x_quantised) return fail(e, DCD_E_INVALID, "internal: pre-quantised operand for a GEMM that does not take the block-scaled path");
+  if (x_quantised && !(fw && e->bf && e->o.gemm_path == 0 && tc_fp8_shape_ok(M, N, K)))
+    return fail(e, DCD_E_INVALID, "internal: pre-quantised operand for a GEMM that takes neither the block-scaled nor the FP8 path");
   if (e->nv4) {
     // The same product by the long route (gemm_path 2, or a shape the native kernel does not take): both operands go through the
     // e2m1/e4m3 round trip; their dequantised values are exact in bf16, so the bf16 tensor-core GEMM
@@ -405,7 +406,7 @@ int gemm(dcd_engine* e, const void* X, const TcTensorMap* tmA, const void* W, co
     w4_stage_used = b;
   }
   if (fw && e->bf && e->o.gemm_path == 0 && tc_fp8_shape_ok(M, N, K)) {
-    {
+    if (!x_quantised) {  // else the norm in front of it left its codes and scales in aq / a_scale
       Scope sc(e, DCD_PROF_ELEMENTWISE, 3.0 * M * (double)K, 1);
       CK(e, launch_quant_fp8_rows<bf16>((const bf16*)X, (size_t)K, e->aq, e->a_scale, M, K, 1.0f, e->stream), "fp8 activation quantisation");
     }
@@ -499,6 +500,11 @@ int run_layers(dcd_engine* e, const Pass& p) {
   // FP8 only in question passes with enough rows; capture and the per-row reference stay bf16
   // (native/src/engine.rs:4321-4326, fp8_min_rows :246-257)
   const bool q8 = e->fp8 && tc && p.mode == 1 && p.T >= e->o.fp8_min_rows;
+  // ... and the norms that feed its projections write e4m3 rows instead of bf16 h (the bits of the norm followed by the quantiser)
+  const bool h8 = q8 && fused_resid && sizeof(T) == 2 && tc_fp8_shape_ok(T_, e->qkv_n, H) && tc_fp8_shape_ok(T_, e->gin_n, H) && tc_fp8_shape_ok(T_, e->gu_rows, H);
+  auto norm8 = [&](const void* x, const void* w) {
+    return launch_rmsnorm_fp8<bf16>((const bf16*)x, (size_t)H, nullptr, 0, (const bf16*)w, nullptr, e->aq, e->a_scale, T_, H, c.rms_eps, true, 1.0f, true, s);
+  };
   TcTensorMap tm_h, tm_A, tm_B, tm_act;
   if (tc) {
     if (tc_make_tmap_a(&tm_h, e->h, T_, H) || tc_make_tmap_a(&tm_A, e->bufA, T_, heads * hd) ||
@@ -514,10 +520,11 @@ int run_layers(dcd_engine* e, const Pass& p) {
     if (li == 0) {
       Scope sc(e, DCD_PROF_ELEMENTWISE, 2.0 * xbytes, 1);
       if (h_fused_quant) CK(e, launch_rmsnorm_nvfp4((const bf16*)e->x, (const bf16*)w.input_norm, e->xq, e->xsft, T_, H, c.rms_eps, s), "rmsnorm + nvfp4");
+      else if (h8) CK(e, norm8(e->x, w.input_norm), "rmsnorm + fp8");
       else CK(e, launch_rmsnorm<T>((const T*)e->x, (const T*)w.input_norm, (T*)e->h, T_, H, c.rms_eps, true, s), "rmsnorm");
     }
     if (w.full) {
-      int rc = gemm<T>(e, e->h, &tm_h, w.w_qkv, &w.tm_qkv, q8 ? &w.f_qkv : nullptr, &w.g_qkv, &w.n_qkv, e->big, T_, e->qkv_n, H, e->qkv_n, 0, h_fused_quant);
+      int rc = gemm<T>(e, e->h, &tm_h, w.w_qkv, &w.tm_qkv, q8 ? &w.f_qkv : nullptr, &w.g_qkv, &w.n_qkv, e->big, T_, e->qkv_n, H, e->qkv_n, 0, h_fused_quant || h8);
       if (!rc) rc = w4_prefetch(e, &w.g_o, T_);
       if (rc) return rc;
       T* big = (T*)e->big;
@@ -579,7 +586,7 @@ int run_layers(dcd_engine* e, const Pass& p) {
       if (!rc) rc = w4_prefetch(e, &w.g_gu, T_);
       if (rc) return rc;
     } else {
-      int rc = gemm<T>(e, e->h, &tm_h, w.w_gin, &w.tm_gin, q8 ? &w.f_gin : nullptr, &w.g_gin, &w.n_gin, e->big, T_, e->gin_n, H, e->gin_n, 0, h_fused_quant);
+      int rc = gemm<T>(e, e->h, &tm_h, w.w_gin, &w.tm_gin, q8 ? &w.f_gin : nullptr, &w.g_gin, &w.n_gin, e->big, T_, e->gin_n, H, e->gin_n, 0, h_fused_quant || h8);
       if (!rc) rc = w4_prefetch(e, &w.g_out, T_);
       if (rc) return rc;
       T* big = (T*)e->big;
@@ -688,6 +695,8 @@ int run_layers(dcd_engine* e, const Pass& p) {
       Scope sc(e, DCD_PROF_ELEMENTWISE, 4.0 * xbytes, 1);
       if (fused_resid && h_fused_quant)
         CK(e, launch_rmsnorm_nvfp4((const bf16*)e->x1, (const bf16*)w.post_norm, e->xq, e->xsft, T_, H, c.rms_eps, s), "rmsnorm + nvfp4");
+      else if (h8)
+        CK(e, norm8(e->x1, w.post_norm), "rmsnorm + fp8");
       else if (fused_resid)
         CK(e, launch_rmsnorm<T>((const T*)e->x1, (const T*)w.post_norm, (T*)e->h, T_, H, c.rms_eps, true, s), "rmsnorm");
       else if (h_fused_quant)
@@ -698,7 +707,7 @@ int run_layers(dcd_engine* e, const Pass& p) {
            "add_rmsnorm");
     }
     if (fused_swiglu) {
-      int rc = gemm<T>(e, e->h, &tm_h, w.w_gu, &w.tm_gu, q8 ? &w.f_gu : nullptr, &w.g_gu, &w.n_gu, e->act, T_, e->gu_rows, H, e->I, 1);
+      int rc = gemm<T>(e, e->h, &tm_h, w.w_gu, &w.tm_gu, q8 ? &w.f_gu : nullptr, &w.g_gu, &w.n_gu, e->act, T_, e->gu_rows, H, e->I, 1, h8);
       if (!rc) rc = w4_prefetch(e, &w.g_down, T_);
       if (rc) return rc;
     } else if (act_epi4) {
@@ -721,6 +730,8 @@ int run_layers(dcd_engine* e, const Pass& p) {
       Scope sc(e, DCD_PROF_ELEMENTWISE, 4.0 * xbytes, 1);
       if (fused_resid && h_fused_quant)
         CK(e, launch_rmsnorm_nvfp4((const bf16*)e->x, (const bf16*)e->layers[li + 1].input_norm, e->xq, e->xsft, T_, H, c.rms_eps, s), "rmsnorm + nvfp4");
+      else if (h8)
+        CK(e, norm8(e->x, e->layers[li + 1].input_norm), "rmsnorm + fp8");
       else if (fused_resid)
         CK(e, launch_rmsnorm<T>((const T*)e->x, (const T*)e->layers[li + 1].input_norm, (T*)e->h, T_, H, c.rms_eps, true, s), "rmsnorm");
       else if (h_fused_quant)
