@@ -1,12 +1,15 @@
 // Attention of the newest tokens of many sequences over their stretches of a 4-bit K/V cache (dcd_k_attention_kv4_decode).
 //
-// A pair is a sequence with one K/V head (and, for more query rows than a CTA holds, one round of them); its keys come in blocks of
-// 32. All blocks of all pairs lie behind each other and every CTA of one resident wave takes the same number of them, so sequences of
-// very different lengths keep every SM busy to the end, and a CTA pays its start (offsets, Q, the first loads: about 8 us, as much as
-// 150 keys' streaming per warp) once or twice instead of once per chunk. A CTA's warps take its blocks in
-// turn, each with a ring of blocks of its own in shared memory (cp.async, no barrier between warps). Few query rows share each key
-// (tokens x heads of the group, eight per MMA column tile), so the kernel lives on getting 0.5625 bytes a value from HBM into
-// matrix fragments:
+// A pair is a sequence with up to four neighbouring K/V heads (and, for more query rows than a warp holds, one round of them); its keys
+// come in blocks of 32. All blocks of all pairs lie behind each other and every CTA of one resident wave takes the same number of
+// them, so sequences of very different lengths keep every SM busy to the end, and a CTA pays its start (offsets, Q, the first loads)
+// once or twice instead of once per chunk of keys. A warp has one of the heads (with fewer than four, the warps of a head take its
+// blocks in turn), so that a CTA reads whole rows of the cache: one head's 128 bytes of every 512, and 16 of every 64 bytes of scales,
+// cost 17 % more DRAM traffic than they hold. Each warp has room for one block of its own in shared memory (cp.async, no barrier between
+// warps): the next K is on its way from the end of the S products on, the next V from the end of the P.V products, so that half a block
+// per warp is always in flight and twelve warps fit on an SM (with two and three whole blocks a warp and eight warps, two thirds of
+// the issue slots stayed empty). Few query rows share each key (tokens x heads of the group, eight per MMA column tile), so the kernel lives on getting
+// 0.5625 bytes a value from HBM into matrix fragments:
 //   S^T[16 keys, 8 rows]  += K[16 keys, 16 dims] Q^T      mma.m16n8k16 with the KEYS as the 16-row operand: all of it is used
 //   O^T[16 dims, 8 rows]  += V^T[16 dims, 16 keys] P^T    even for one token of six heads, where rows as M would fill 6 of 16
 // The fragments are made in registers straight from the code words. The order of the contracted dimensions is free as long as Q has
@@ -22,6 +25,8 @@
 //
 // A pair that lies in one CTA is finished there; the parts of one that is cut leave their unnormalised O with maximum and sum in the
 // workspace, and a second kernel adds them up in their order. Keys beyond the stretch are zero-filled, masked keys get p = 0.
+#include <type_traits>
+
 #include "common.cuh"
 #include "kv4.h"
 
@@ -30,15 +35,14 @@ namespace kvd {
 constexpr int KB = 32;
 constexpr float P_SHIFT = 10.0f;  // P is held as p * 2^10
 
-// Warps of a CTA, blocks in a warp's ring, CTAs per SM, Q fragments in shared memory instead of registers
+constexpr int WARPS = 4;
+// CTAs per SM, Q fragments in shared memory where registers run out
 template <int HD, int NT> struct Cfg {
-  static constexpr int WARPS = HD == 256 && NT == 1 ? 6 : 4;
-  static constexpr int STAGES = HD == 256 && NT == 1 ? 2 : 3;
-  static constexpr int CTAS = HD == 256 ? (NT == 1 ? 2 : 1) : NT == 1 ? 3 : 2;
+  static constexpr int CTAS = NT == 1 ? 3 : 2;
   static constexpr bool Q_SMEM = NT * HD >= 256;
 };
 
-template <int HD> struct Ring {
+template <int HD> struct Block {
   static constexpr int ROW = HD / 2, SROW = HD / 16;                            // bytes of a key's codes and scales
   static constexpr int K = 0, V = KB * ROW, KS = 2 * KB * ROW, VS = KS + KB * SROW;
   static constexpr int BYTES = VS + KB * SROW;
@@ -100,6 +104,7 @@ template <int HD> __device__ __forceinline__ int v_chunk(int k, int c) { return 
 
 struct Args {
   Kv4DecodeArgs a;
+  int hc;          // K/V heads of a pair: 4, 2 or 1
   int q_min;       // least blocks per CTA
   int max_parts;   // parts of a pair, at most: max_len in blocks / q_min, and one more for its offset
   float* ws_o;     // [T * heads][max_parts][hd]
@@ -131,6 +136,11 @@ __device__ __forceinline__ Sequence sequence(const Kv4DecodeArgs& a, int b, bool
   return s;
 }
 
+// Block numbers are 64-bit; what is divided in earnest fits 32, where a division is a tenth of the 64-bit one.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return (((unsigned long long)a | (unsigned long long)b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 template <int ROWS>
 __device__ __forceinline__ int rounds_of(const Sequence& s, int G) { return (s.L * G + ROWS - 1) / ROWS; }
 // Blocks of one pair of the sequence: at least one, so that the tokens of an empty stretch get their zeros.
@@ -155,21 +165,21 @@ __device__ __forceinline__ void store_row(const Kv4DecodeArgs& a, const float (&
 }
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(Cfg<HD, NT>::WARPS * 32, Cfg<HD, NT>::CTAS) kv4_decode_kernel(const Args p) {
-  using R = Ring<HD>;
+__global__ void __launch_bounds__(WARPS * 32, Cfg<HD, NT>::CTAS) kv4_decode_kernel(const Args p) {
+  using R = Block<HD>;
   constexpr int KW = HD / 32;               // K code words of a lane per key
   constexpr int KL = KW < 4 ? KW : 4;       // ... loaded at once
   constexpr int VW = HD / 64;               // V code words of a lane per key
   constexpr int ROWS = 8 * NT;
-  constexpr int WARPS = Cfg<HD, NT>::WARPS, STAGES = Cfg<HD, NT>::STAGES;
   constexpr bool Q_SMEM = Cfg<HD, NT>::Q_SMEM;
   const Kv4DecodeArgs& a = p.a;
   const int G = a.heads / a.kv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int hc = p.hc, n_groups = a.kv / hc, my_head = warp % hc, first = warp / hc, step = WARPS / hc;  // this warp's head of a pair, and its blocks
   extern __shared__ __align__(16) uint8_t smem[];
-  uint8_t* ring = smem + warp * (STAGES * R::BYTES);
-  const uint32_t ring_addr = smem_addr(ring);
-  uint2* q_smem = reinterpret_cast<uint2*>(smem + WARPS * STAGES * R::BYTES);  // [word * 2 + half][nt][lane]
+  uint8_t* const st = smem + warp * R::BYTES;
+  const uint32_t st_addr = smem_addr(st);
+  uint2* q_smem = reinterpret_cast<uint2*>(smem + WARPS * R::BYTES) + warp * (HD / 16 * NT * 32);  // [word * 2 + half][nt][lane]
   const float scale_log2e = (1.0f / sqrtf((float)HD)) * 1.4426950408889634f;
 
   // ---- this CTA's blocks: thread t adds up the sequences [t * per, (t + 1) * per), then a scan over the threads ------------------------------
@@ -183,7 +193,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::WARPS * 32, Cfg<HD, NT>::CTAS) kv
     long long mine = 0;
     for (int i = b0; i < b1; ++i) {
       const Sequence s = sequence(a, i, blockIdx.x == 0);
-      mine += (long long)a.kv * rounds_of<ROWS>(s, G) * blocks_of(s);
+      mine += (long long)n_groups * rounds_of<ROWS>(s, G) * blocks_of(s);
     }
     long long before = mine, total = 0;
 #pragma unroll
@@ -199,7 +209,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::WARPS * 32, Cfg<HD, NT>::CTAS) kv
       if (i < warp) before += sums[i];
       total += sums[i];
     }
-    quota = max((total + gridDim.x - 1) / (long long)gridDim.x, (long long)p.q_min);
+    quota = max(quotient(total + gridDim.x - 1, gridDim.x), (long long)p.q_min);
     u = quota * blockIdx.x;
     u_end = min(total, u + quota);
     if (u >= u_end) return;
@@ -207,7 +217,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::WARPS * 32, Cfg<HD, NT>::CTAS) kv
       int i = b0;
       for (; i < b1; ++i) {
         const Sequence s = sequence(a, i, false);
-        const long long n = (long long)a.kv * rounds_of<ROWS>(s, G) * blocks_of(s);
+        const long long n = (long long)n_groups * rounds_of<ROWS>(s, G) * blocks_of(s);
         if (u < before + n) break;
         before += n;
       }
@@ -223,15 +233,15 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::WARPS * 32, Cfg<HD, NT>::CTAS) kv
   while (u < u_end) {
     const int nblk = blocks_of(sq), n_rows = sq.L * G;
     const long long in_seq = u - seq_u;
-    if (in_seq >= (long long)a.kv * rounds_of<ROWS>(sq, G) * nblk) {
-      seq_u += (long long)a.kv * rounds_of<ROWS>(sq, G) * nblk;
+    if (in_seq >= (long long)n_groups * rounds_of<ROWS>(sq, G) * nblk) {
+      seq_u += (long long)n_groups * rounds_of<ROWS>(sq, G) * nblk;
       sq = sequence(a, ++b, false);
       continue;
     }
-    const int pair = (int)(in_seq / nblk), kh = pair % a.kv, r0 = pair / a.kv * ROWS, first_blk = (int)(in_seq - (long long)pair * nblk);
+    const int pair = (int)quotient(in_seq, nblk), kh = pair % n_groups * hc + my_head, r0 = pair / n_groups * ROWS, first_blk = (int)(in_seq - (long long)pair * nblk);
     const int n_blocks = (int)min((long long)(nblk - first_blk), u_end - u);
     const long long pair_u = u - first_blk;
-    const int n_parts = (int)((pair_u + nblk - 1) / quota - pair_u / quota) + 1, part = (int)blockIdx.x - (int)(pair_u / quota);
+    const int first_cta = (int)quotient(pair_u, quota), n_parts = (int)quotient(pair_u + nblk - 1, quota) - first_cta + 1, part = (int)blockIdx.x - first_cta;
     u += n_blocks;
     const int k0 = first_blk * KB, k1 = min(sq.len, k0 + n_blocks * KB);  // the keys of this part, relative to the stretch
 
@@ -243,30 +253,40 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::WARPS * 32, Cfg<HD, NT>::CTAS) kv
     const uint8_t* vs = a.cache.v.scales + row0 * R::SROW;
     const size_t code_step = (size_t)a.kv * R::ROW, scale_step = (size_t)a.kv * R::SROW;
 
-  auto fetch = [&](int blk, int slot) {
-    const int j0 = blk * KB, left = (k1 - k0) - j0;  // keys of the block that exist
-    const uint32_t base = ring_addr + slot * R::BYTES;
-    constexpr int CH = R::ROW / 16;
+    // K or V of a block: lane (key, chunk) takes every KPL-th key's 16 bytes; addresses advance by additions
+    constexpr int CHUNKS = R::ROW / 16, KPL = 32 / CHUNKS;
+    const int f_key = lane / CHUNKS, f_chunk = lane % CHUNKS;
+    const size_t lane_code = f_key * code_step + f_chunk * 16, lane_scale = lane * scale_step, pass_step = KPL * code_step;
+    auto fetch = [&](int blk, bool second) {
+      const int left = (k1 - k0) - blk * KB;  // keys of the block that exist
+      const uint8_t* codes = (second ? vc : kc) + (size_t)blk * KB * code_step;
+      const uint8_t* scales = (second ? vs : ks) + (size_t)blk * KB * scale_step;
+      const uint32_t to = st_addr + (second ? R::V : R::K), to_scales = st_addr + (second ? R::VS : R::KS) + lane * R::SROW;
+      const uint8_t* from = codes + lane_code;
+      if (left >= KB) {
 #pragma unroll
-    for (int i = 0; i < KB * CH / 32; ++i) {
-      const int id = lane + 32 * i, key = id / CH, ch = id % CH;
-      const bool ok = key < left;
-      const size_t at = (size_t)(ok ? j0 + key : 0) * code_step + ch * 16;
-      cp_async<16>(base + R::K + key * R::ROW + k_chunk<HD>(key, ch) * 16, kc + at, ok);
-      cp_async<16>(base + R::V + key * R::ROW + v_chunk<HD>(key, ch) * 16, vc + at, ok);
-    }
-    const bool ok = lane < left;  // one key's scales per lane
-    const size_t at = (size_t)(ok ? j0 + lane : 0) * scale_step;
-    cp_async<R::SROW>(base + R::KS + lane * R::SROW, ks + at, ok);
-    cp_async<R::SROW>(base + R::VS + lane * R::SROW, vs + at, ok);
-  };
+        for (int i = 0; i < KB / KPL; ++i) {
+          const int key = i * KPL + f_key;
+          cp_async<16>(to + key * R::ROW + (second ? v_chunk<HD>(key, f_chunk) : k_chunk<HD>(key, f_chunk)) * 16, from, true);
+          from += pass_step;
+        }
+        cp_async<R::SROW>(to_scales, scales + lane_scale, true);
+      } else {  // zeros behind the last key
+#pragma unroll 1
+        for (int i = 0; i < KB / KPL; ++i) {
+          const int key = i * KPL + f_key;
+          cp_async<16>(to + key * R::ROW + (second ? v_chunk<HD>(key, f_chunk) : k_chunk<HD>(key, f_chunk)) * 16, key < left ? from : codes, key < left);
+          from += pass_step;
+        }
+        cp_async<R::SROW>(to_scales, lane < left ? scales + lane_scale : scales, lane < left);
+      }
+    };
 
-    // ---- the first blocks are on their way before Q is read -----------------------------------------
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-      if (warp + i * WARPS < n_blocks) fetch(warp + i * WARPS, i);
-      cp_commit();
-    }
+    // ---- the first block is on its way before Q is read -----------------------------------------
+    if (first < n_blocks) fetch(first, false);
+    cp_commit();
+    if (first < n_blocks) fetch(first, true);
+    cp_commit();
     // ---- Q as the column operand: lane (g, c) holds row g's dimensions of quad position c -------------
     uint2 qf[Q_SMEM ? 1 : NT][Q_SMEM ? 1 : KW * 2];
     float f[NT][2];  // softmax factor of rows 2c, 2c + 1
@@ -298,10 +318,8 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::WARPS * 32, Cfg<HD, NT>::CTAS) kv
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = pack_f16(__low2float(h[i]) * inv, __high2float(h[i]) * inv);
         if constexpr (Q_SMEM) {
-          if (warp == 0) {
-            q_smem[((2 * w) * NT + nt) * 32 + lane] = make_uint2(v[0], v[1]);
-            q_smem[((2 * w + 1) * NT + nt) * 32 + lane] = make_uint2(v[2], v[3]);
-          }
+          q_smem[((2 * w) * NT + nt) * 32 + lane] = make_uint2(v[0], v[1]);
+          q_smem[((2 * w + 1) * NT + nt) * 32 + lane] = make_uint2(v[2], v[3]);
         } else {
           qf[nt][2 * w] = make_uint2(v[0], v[1]);
           qf[nt][2 * w + 1] = make_uint2(v[2], v[3]);
@@ -316,7 +334,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::WARPS * 32, Cfg<HD, NT>::CTAS) kv
         end[nt][i] = min(sq.len - (sq.L - 1 - rr / G), k1) - k0;
       }
     }
-    if constexpr (Q_SMEM) __syncthreads();
+    if constexpr (Q_SMEM) __syncwarp();
 
     float o[HD / 16][NT][4];
 #pragma unroll
@@ -336,14 +354,9 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::WARPS * 32, Cfg<HD, NT>::CTAS) kv
         first_end = min(first_end, end[nt][i]);
       }
 
-    int slot = 0;
-    for (int blk = warp; blk < n_blocks; blk += WARPS) {
-      if (blk + (STAGES - 1) * WARPS < n_blocks) fetch(blk + (STAGES - 1) * WARPS, slot == 0 ? STAGES - 1 : slot - 1);
-      cp_commit();
-      cp_wait<STAGES - 1>();
+    for (int blk = first; blk < n_blocks; blk += step) {
+      cp_wait<1>();  // K; V may still be under way
       __syncwarp();
-      const uint8_t* st = ring + slot * R::BYTES;
-
       // ---- S^T of two 16-key tiles ------------------------------------------------------------------
       float s[2][NT][4];
 #pragma unroll
@@ -390,6 +403,10 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::WARPS * 32, Cfg<HD, NT>::CTAS) kv
             }
         }
       }
+
+      __syncwarp();
+      if (blk + step < n_blocks) fetch(blk + step, false);
+      cp_commit();
 
       // ---- softmax: lane (g, c) has keys g, g + 8 of either tile for rows 2c, 2c + 1 --------------------
       const int j0 = blk * KB;
@@ -440,9 +457,17 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::WARPS * 32, Cfg<HD, NT>::CTAS) kv
         }
       }
 
+      cp_wait<1>();  // V; the next K may still be under way
+      __syncwarp();
       // ---- O^T += V^T P^T: lane (g, c) holds 8 to 32 dimensions of keys 2c, 2c + 1, 2c + 8, 2c + 9 ---------
-#pragma unroll
+#pragma unroll 1
       for (int t = 0; t < 2; ++t) {
+        uint32_t pt[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          pt[nt][0] = t ? pb[1][nt][0] : pb[0][nt][0];
+          pt[nt][1] = t ? pb[1][nt][1] : pb[0][nt][1];
+        }
         uint32_t w[4][VW], sc[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -483,21 +508,23 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::WARPS * 32, Cfg<HD, NT>::CTAS) kv
           for (int j = 0; j < 4; ++j) {
             const uint32_t a0 = hmul(ev[j], sa), a1 = hmul(ov[j], sa), a2 = hmul(ev8[j], sb), a3 = hmul(ov8[j], sb);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma(o[wi * 4 + j][nt], a0, a1, a2, a3, pb[t][nt][0], pb[t][nt][1]);
+            for (int nt = 0; nt < NT; ++nt) mma(o[wi * 4 + j][nt], a0, a1, a2, a3, pt[nt][0], pt[nt][1]);
           }
         }
       }
-      __syncwarp();  // the slot may be refilled
-      slot = slot + 1 == STAGES ? 0 : slot + 1;
+      __syncwarp();
+      if (blk + step < n_blocks) fetch(blk + step, true);
+      cp_commit();
     }
     cp_wait<0>();
-    __syncthreads();  // the rings are free: they take the warps' parts
+    __syncthreads();  // the blocks are done with: the warps' parts take their place
 
     // ---- the four warps' parts of each row. Dimension g * (HD / 8) + 2 t + e lies at t * 16 + 2 g + e, and rows are HD + 4 floats
     // apart: the sixteen lanes of a store (four g, four rows two apart) then meet sixteen different pairs of banks ----------------
     constexpr int PITCH = HD + 4;
     float* part_o = reinterpret_cast<float*>(smem);                                // [warp][row][PITCH]
     float2* part_ml = reinterpret_cast<float2*>(smem + WARPS * ROWS * PITCH * 4);  // [warp][row]
+    float2* total_ml = part_ml + WARPS * ROWS;                                     // [row][head]
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -512,61 +539,99 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::WARPS * 32, Cfg<HD, NT>::CTAS) kv
         for (int t = 0; t < HD / 16; ++t) *reinterpret_cast<float2*>(dst + 16 * t) = make_float2(o[t][nt][i], o[t][nt][i + 2]);
       }
     __syncthreads();
-    const int rows_here = min(ROWS, n_rows - r0);
-    constexpr int PER = HD / 32;  // consecutive values of a lane; one warp per row
-    const int d0 = lane * PER, at0 = d0 % (HD / 8) * 8 + d0 / (HD / 8) * 2;
-    for (int row = warp; row < rows_here; row += WARPS) {
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, part_ml[w * ROWS + row].x);
-      float acc[PER], sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
+    // every (head, row): the maximum and sum over the head's warps hs, hs + hc, ..., and the warps' weights in place of their maxima
+    const int rows_here = min(ROWS, n_rows - r0), n_out = rows_here * hc;
+    for (int i = threadIdx.x; i < n_out; i += WARPS * 32) {
+      const int row = i / hc, hs = i - row * hc;
+      float M = -INFINITY, sum = 0.f;
+      for (int w = hs; w < WARPS; w += hc) M = fmaxf(M, part_ml[w * ROWS + row].x);
+      for (int w = hs; w < WARPS; w += hc) {
         const float2 ml = part_ml[w * ROWS + row];
         const float fw = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
         sum += fw * ml.y;
+        part_ml[w * ROWS + row].x = fw;
+      }
+      total_ml[i] = make_float2(M, sum);
+    }
+    __syncthreads();
+    constexpr int PER = HD / 32;  // consecutive values of a lane; one warp per row
+    const int d0 = lane * PER, at0 = d0 % (HD / 8) * 8 + d0 / (HD / 8) * 2;
+    // WK warps of a head, IL rows of a warp at a time
+    auto rows_out = [&](auto wk, auto il) {
+      constexpr int WK = decltype(wk)::value, IL = decltype(il)::value;
+      for (int i0 = warp; i0 < n_out; i0 += WARPS * IL) {
+        float acc[IL][PER];
+        int hs[IL], row[IL];
 #pragma unroll
-        for (int i = 0; i < PER; i += 2) {
-          const float2 v = *reinterpret_cast<const float2*>(part_o + (w * ROWS + row) * PITCH + at0 + 8 * i);
-          acc[i] += fw * v.x;
-          acc[i + 1] += fw * v.y;
+        for (int n = 0; n < IL; ++n) {
+          const int i = min(i0 + n * WARPS, n_out - 1);
+          row[n] = i / (WARPS / WK);
+          hs[n] = i % (WARPS / WK);
+#pragma unroll
+          for (int j = 0; j < PER; ++j) acc[n][j] = 0.f;
+#pragma unroll
+          for (int v = 0; v < WK; ++v) {
+            const int w = hs[n] + v * (WARPS / WK);
+            const float fw = part_ml[w * ROWS + row[n]].x;
+#pragma unroll
+            for (int j = 0; j < PER; j += 2) {
+              const float2 x = *reinterpret_cast<const float2*>(part_o + (w * ROWS + row[n]) * PITCH + at0 + 8 * j);
+              acc[n][j] += fw * x.x;
+              acc[n][j + 1] += fw * x.y;
+            }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < IL; ++n) {
+          const int i = i0 + n * WARPS;
+          if (i >= n_out) break;
+          const float2 ml = total_ml[i];
+          const int r = r0 + row[n], tt = r / G, t = sq.off + tt, h = (kh - my_head + hs[n]) * G + r - tt * G;
+          const size_t at = (size_t)t * a.heads + h;
+          if (part == 0 && lane == 0) p.ws_n[at] = n_parts;
+          if (n_parts > 1) {
+            if (lane == 0) p.ws_ml[at * p.max_parts + part] = ml;
+            float* dst = p.ws_o + (at * p.max_parts + part) * HD + d0;
+#pragma unroll
+            for (int j = 0; j < PER; j += 2) *reinterpret_cast<float2*>(dst + j) = make_float2(acc[n][j], acc[n][j + 1]);
+          } else {
+            store_row<PER>(a, acc[n], ml.y, at, t, h, HD, d0);
+          }
         }
       }
-      const int r = r0 + row, t = sq.off + r / G, h = kh * G + r % G;
-      const size_t at = (size_t)t * a.heads + h;
-      if (part == 0 && lane == 0) p.ws_n[at] = n_parts;
-      if (n_parts > 1) {
-        if (lane == 0) p.ws_ml[at * p.max_parts + part] = make_float2(M, sum);
-        float* dst = p.ws_o + (at * p.max_parts + part) * HD + d0;
-#pragma unroll
-        for (int i = 0; i < PER; i += 2) *reinterpret_cast<float2*>(dst + i) = make_float2(acc[i], acc[i + 1]);
-      } else {
-        store_row<PER>(a, acc, sum, at, t, h, HD, d0);
-      }
-    }
-    if (u < u_end) __syncthreads();  // before the rings are filled again
+    };
+    if (hc == 4) rows_out(std::integral_constant<int, 1>(), std::integral_constant<int, HD == 256 ? 3 : 4>());
+    else if (hc == 2) rows_out(std::integral_constant<int, 2>(), std::integral_constant<int, HD == 256 ? 3 : 4>());
+    else rows_out(std::integral_constant<int, 4>(), std::integral_constant<int, 2>());
+    if (u < u_end) __syncthreads();  // before the next pair's blocks come
   }
 }
 
-// out = sum_z O_z 2^(m_z - M) / sum_z l_z 2^(m_z - M): one warp per (token, head), the parts in their order
-template <int HD>
+// out = sum_z O_z 2^(m_z - M) / sum_z l_z 2^(m_z - M). W warps per (token, head) take the parts in turn; their sums are added in
+// order. The row's sequence is found 32 offsets at a time, and 32 parts' weights come at once, so that little of the kernel is a chain
+// of loads (one after the other they were 28 us for one token over 64 parts).
+template <int HD, int W>
 __global__ void __launch_bounds__(128) kv4_decode_merge_kernel(const Args p) {
   constexpr int PER = HD / 32;
+  __shared__ float part[W > 1 ? 4 : 1][HD], part_sum[4];
   const Kv4DecodeArgs& a = p.a;
-  const size_t at = (size_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, t = (int)(at / (unsigned)a.heads), h = (int)(at - (size_t)t * a.heads);
-  if (t >= a.T || t >= a.cu[a.B]) return;
-  int lo = 0, hi = a.B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu[mid] <= t) lo = mid; else hi = mid;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = warp % W;
+  const size_t at = (size_t)blockIdx.x * (4 / W) + warp / W;
+  const int t = (int)(at / (unsigned)a.heads), h = (int)(at - (size_t)t * a.heads);
+  int nz = 0;
+  if (t < a.T) {
+    int lo = 0, hi = a.B;  // cu[lo] <= t, and t < cu[hi] where it is in a sequence at all
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32, i = min(lo + (lane + 1) * step, hi);
+      const unsigned below = __ballot_sync(0xffffffffu, i < hi && a.cu[i] <= t);
+      const int n = __popc(below);  // offsets rise
+      hi = min(lo + (n + 1) * step, hi);
+      lo += n * step;
+    }
+    const int off = a.cu[lo], end = a.cu[lo + 1];
+    if (off >= 0 && off <= t && t < end && end <= a.T) nz = p.ws_n[at];
   }
-  const Sequence sq = sequence(a, lo, false);
-  if (sq.L == 0) return;
-  const int nz = p.ws_n[at];
-  if (nz == 1) return;  // finished by its only CTA
+  if (W == 1 && nz <= 1) return;  // finished by its only CTA, or no token of a sequence
   const float2* ml = p.ws_ml + at * p.max_parts;
   float M = -INFINITY;
   for (int z = lane; z < nz; z += 32) M = fmaxf(M, ml[z].x);
@@ -574,19 +639,41 @@ __global__ void __launch_bounds__(128) kv4_decode_merge_kernel(const Args p) {
   float acc[PER], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-  if (M != -INFINITY) {
+  if (nz > 1 && M != -INFINITY) {
     const float* src = p.ws_o + at * p.max_parts * HD + lane * PER;
-#pragma unroll 4
-    for (int z = 0; z < nz; ++z) {
-      const float2 x = ml[z];
-      const float w = ex2(x.x - M);  // a part that saw nothing has m = -inf: weight 0 on zeros
-      sum += w * x.y;
+    for (int z0 = w; z0 < nz; z0 += 32 * W) {  // this warp's next 32 parts: z0, z0 + W, ...
+      const int mine = z0 + lane * W;
+      const float2 x = mine < nz ? ml[mine] : make_float2(-INFINITY, 0.f);
+      const float wt = ex2(x.x - M);  // a part that saw nothing has m = -inf: weight 0 on zeros
+      sum += wt * x.y;
+      const int n = min(32, (nz - z0 + W - 1) / W);
+#pragma unroll 8
+      for (int z = 0; z < n; ++z) {
+        const float wz = __shfl_sync(0xffffffffu, wt, z);
 #pragma unroll
-      for (int i = 0; i < PER; i += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(src + (size_t)z * HD + i);
-        acc[i] += w * v.x;
-        acc[i + 1] += w * v.y;
+        for (int i = 0; i < PER; i += 2) {
+          const float2 v = *reinterpret_cast<const float2*>(src + (size_t)(z0 + z * W) * HD + i);
+          acc[i] += wz * v.x;
+          acc[i + 1] += wz * v.y;
+        }
       }
+    }
+    sum = warp_sum(sum);
+  }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) part[warp][lane * PER + i] = acc[i];
+    if (lane == 0) part_sum[warp] = sum;
+    __syncthreads();
+    if (w != 0 || nz <= 1) return;
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+#pragma unroll
+    for (int v = 0; v < W; ++v) {
+      sum += part_sum[warp + v];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) acc[i] += part[warp + v][lane * PER + i];
     }
   }
   store_row<PER>(a, acc, sum, at, t, h, HD, lane * PER);
@@ -598,31 +685,33 @@ int sm_count() {
   return sms;
 }
 
-// The number of CTAs (two per SM are resident), the least blocks that one takes (one per warp, and not so few that the parts of a pair
-// outgrow the workspace where most sequences are far shorter than max_len), and the parts that a pair can then have.
+// The K/V heads of a pair, the SMs, the least blocks that a CTA takes (two per warp, and not so few that the parts of a pair outgrow the
+// workspace where most sequences are far shorter than max_len), and the parts that a pair can then have.
 struct Plan {
-  int ctas, q_min, max_parts;
+  int hc, sms, q_min, max_parts;
 };
 Plan plan_of(int B, int kv, int max_len) {
   Plan p;
-  p.ctas = sm_count();
-  const long long blocks = max(1, (int)(((long long)max_len + KB - 1) / KB));
-  p.q_min = (int)max(4LL, ((long long)B * kv * blocks / (2 * p.ctas) + 3) / 4);
+  p.hc = kv % 4 == 0 ? 4 : kv % 2 == 0 ? 2 : 1;
+  p.sms = sm_count();
+  const long long blocks = max(1LL, ((long long)max_len + KB - 1) / KB);
+  p.q_min = (int)max(2LL * WARPS / p.hc, ((long long)B * (kv / p.hc) * blocks / (2 * p.sms) + 3) / 4);
   p.max_parts = (int)((blocks + p.q_min - 1) / p.q_min) + 1;
   return p;
 }
 
 template <int HD, int NT>
-cudaError_t run(const Args& p, int ctas, cudaStream_t s) {
+cudaError_t run(const Args& p, int sms, cudaStream_t s) {
   using C = Cfg<HD, NT>;
-  constexpr int rings = C::WARPS * C::STAGES * Ring<HD>::BYTES + (C::Q_SMEM ? HD / 16 * NT * 256 : 0), parts = C::WARPS * 8 * NT * ((HD + 4) * 4 + 8);
-  constexpr int bytes = rings > parts ? rings : parts;
+  constexpr int blocks = WARPS * (Block<HD>::BYTES + (C::Q_SMEM ? HD / 16 * NT * 256 : 0)), parts = WARPS * 8 * NT * ((HD + 4) * 4 + 16);
+  constexpr int bytes = blocks > parts ? blocks : parts;
   static_assert(C::CTAS * (bytes + 1024 + 256) <= 228 * 1024, "shared memory of an SM");
   CUDA_TRY(cudaFuncSetAttribute(kv4_decode_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  kv4_decode_kernel<HD, NT><<<ctas * C::CTAS, C::WARPS * 32, bytes, s>>>(p);
+  kv4_decode_kernel<HD, NT><<<sms * C::CTAS, WARPS * 32, bytes, s>>>(p);
   CUDA_TRY(cudaGetLastError());
   const size_t rows = (size_t)p.a.T * p.a.heads;
-  kv4_decode_merge_kernel<HD><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
+  if (p.max_parts <= 8) kv4_decode_merge_kernel<HD, 1><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
+  else kv4_decode_merge_kernel<HD, 4><<<(unsigned)rows, 128, 0, s>>>(p);
   return cudaGetLastError();
 }
 
@@ -638,13 +727,14 @@ cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, void* workspace, cudaStrea
   const size_t parts = (size_t)a.T * a.heads * plan.max_parts;
   kvd::Args p;
   p.a = a;
+  p.hc = plan.hc;
   p.q_min = plan.q_min;
   p.max_parts = plan.max_parts;
   p.ws_o = (float*)workspace;
   p.ws_ml = (float2*)(p.ws_o + parts * a.hd);
   p.ws_n = (int*)(p.ws_ml + parts);
   // column tiles of eight rows by the rows of a sequence of average length; longer ones take several rounds over their keys
-  const int rows = ((a.T + a.B - 1) / a.B) * (a.heads / a.kv), n = plan.ctas;
+  const int rows = ((a.T + a.B - 1) / a.B) * (a.heads / a.kv), n = plan.sms;
   if (a.hd == 256) return rows <= 8 ? kvd::run<256, 1>(p, n, s) : kvd::run<256, 2>(p, n, s);
   if (a.hd == 128) return rows <= 8 ? kvd::run<128, 1>(p, n, s) : rows <= 16 ? kvd::run<128, 2>(p, n, s) : kvd::run<128, 4>(p, n, s);
   return rows <= 8 ? kvd::run<64, 1>(p, n, s) : rows <= 16 ? kvd::run<64, 2>(p, n, s) : kvd::run<64, 4>(p, n, s);

@@ -331,7 +331,7 @@ int dcd_k_attention_kv4(const void* q, size_t q_stride, const void* k_own, size_
                         void* stream) {
   if (B <= 0 || T <= 0 || n_state < 0 || !heads_ok(heads, kv, hd)) return DCD_E_INVALID;
   if (!rows_ok(q, q_stride, (size_t)heads * hd) || !rows_ok(k_own, k_stride, (size_t)kv * hd) || !rows_ok(v_own, v_stride, (size_t)kv * hd)) return DCD_E_INVALID;
-  if ((n_state > 0 && !cache_ok(k_codes, k_scales, v_codes, v_scales)) || (gate_qg && !rows_ok(gate_qg, qg_stride, (size_t)2 * heads * hd))) return DCD_E_INVALID;
+  if ((n_state > 0 && !cache_ok(k_codes, k_scales, v_codes, v_scales)) || (gate_qg && (!rows_ok(gate_qg, qg_stride, (size_t)2 * heads * hd) || qg_stride > (1u << 24)))) return DCD_E_INVALID;
   if (!out || reinterpret_cast<uintptr_t>(out) % 16 != 0 || !cu_seqlens) return DCD_E_INVALID;
   const size_t need = kv4_question_workspace(B, T, n_state, heads, kv, hd);
   if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)) return DCD_E_INVALID;
@@ -350,7 +350,7 @@ int dcd_k_attention_kv4_decode(const void* q, size_t q_stride, const void* k_cod
                                const int32_t* cu_seqlens, int B, int T, int heads, int kv, int hd, void* workspace, size_t workspace_bytes, int* err,
                                void* stream) {
   if (B <= 0 || T <= 0 || max_len < 0 || max_len > (1 << 30) || !heads_ok(heads, kv, hd) || !rows_ok(q, q_stride, (size_t)heads * hd)) return DCD_E_INVALID;
-  if (!cache_ok(k_codes, k_scales, v_codes, v_scales) || !seg_start || !seg_len || (gate_qg && !rows_ok(gate_qg, qg_stride, (size_t)2 * heads * hd))) return DCD_E_INVALID;
+  if (!cache_ok(k_codes, k_scales, v_codes, v_scales) || !seg_start || !seg_len || (gate_qg && (!rows_ok(gate_qg, qg_stride, (size_t)2 * heads * hd) || qg_stride > (1u << 24)))) return DCD_E_INVALID;
   if (!out || reinterpret_cast<uintptr_t>(out) % 16 != 0 || !cu_seqlens) return DCD_E_INVALID;
   const size_t need = kv4_decode_workspace(B, T, max_len, heads, kv, hd);
   if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)) return DCD_E_INVALID;

@@ -685,7 +685,7 @@ DCD_API int dcd_k_kv4_read(const void* k_codes, const void* k_scales, const void
  * of them, or with causal != 0 those up to itself), out = softmax(q k / sqrt(hd)) v, times sigmoid(gate) where gate_qg (laid out as
  * there) is given. n_state 0 with causal 1 is causal attention over packed prompts; the cache pointers may then be NULL. bf16; any
  * heads that kv divides; hd 64, 128 or 256; q [T, heads, hd], k_own and v_own [T, kv, hd] with row strides in elements, multiples of 8,
- * 16-byte aligned; out [T, heads, hd]. cu_seqlens [B + 1] rises from 0 to at most T; rows of out behind the last sequence
+ * 16-byte aligned, qg_stride at most 2^24; out [T, heads, hd]. cu_seqlens [B + 1] rises from 0 to at most T; rows of out behind the last sequence
  * are left as they were. workspace: dcd_k_attention_kv4_workspace bytes (0: none is needed), 16-byte aligned, not shared by calls that
  * may overlap. */
 DCD_API size_t dcd_k_attention_kv4_workspace(int B, int T, int n_state, int heads, int kv, int hd);
