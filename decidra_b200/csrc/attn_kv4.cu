@@ -19,8 +19,8 @@
 // a second issuing warp S[j + 2] and P.V[j + 1] share the tensor core, and the loop S, softmax, P.V of a tile gets longer by that:
 // slower.) K and V come through one ring of 32 KB slots (16 KB at head_dim 64, a whole tile) in the order in which they are used, so that
 // the loads run two and more product phases ahead. A barrier wait that is already satisfied still takes 100 to 170 cycles, which made
-// the issuing warp slower than the tensor core (2048 cycles a tile at head_dim 256: 4360 with 16 KB slots, 3080 with 32 KB), so it asks
-// for the next barrier's state before it issues the products of the present one.
+// the issuing warp slower than the tensor core (2048 cycles a tile at head_dim 256: 4360 with 16 KB slots, 3080 with 32 KB), so another
+// warp waits in its place (364 -> 330 us over 64 questions of about 107 tokens and 2048 state rows).
 // The rows of O leave through a ring slot too: lane = row in TMEM, and sixteen bytes a row would be 32 lines a store; staged, a
 // store covers four rows of 64 bytes.
 //
@@ -41,7 +41,7 @@ namespace kvq {
 using namespace tcc;
 
 constexpr int KT = 128;                   // keys of a tile
-constexpr int NUM_THREADS = 320, ISSUER = 8, LOADER = 9;
+constexpr int NUM_THREADS = 352, ISSUER = 8, LOADER = 9, WAITER = 10;  // warps 0-7: softmax and epilogue
 constexpr int MAX_ITEMS = 64;             // work items of a CTA
 constexpr uint32_t S_COL = 256;           // TMEM: O from column 0, S at 256 and 384
 constexpr float RESCALE = 8.0f;           // log2 units
@@ -151,20 +151,9 @@ struct Keys {
   }
 };
 
-// Whether the phase of that parity is complete, without waiting.
-__device__ __forceinline__ uint32_t mbar_test(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n"
-      ".reg .pred p;\n"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-      "selp.u32 %0, 1, 0, p;\n"
-      "}\n"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok;
-}
+constexpr int EVENTS = 14;  // hardware barriers 1 to 14
+__device__ __forceinline__ void named_sync(int id) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void named_arrive(int id) { asm volatile("barrier.cta.arrive %0, 64;" ::"r"(id) : "memory"); }
 
 // Predicated instructions: a branch around each of a lane's rows costs more than the access
 __device__ __forceinline__ uint2 ld_global_if(const void* p, bool there) {
@@ -353,44 +342,72 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       advance();
       ++live;
     }
+  } else if (warp == WAITER) {
+    // ---- waits for the issuer: the same barriers in the same order, each handed on through a hardware barrier. A satisfied mbarrier wait
+    // takes 100 to 170 cycles, the hardware barrier 20 to 30; the tensor core's queue holds two or three products, so that what the
+    // issuing warp waits is lost. V's slots are waited for in front of P, which comes last, and share its event. At most the ring's
+    // slots and two P are announced ahead, fewer than there are EVENTS. A wait that gave up is still announced, with the flag up, and
+    // nothing after it ----------------------------------------------------------------------------------------------------------
+    bool ok = true;
+    int slot = 0, jj = 0;
+    uint32_t use = 0, event = 0;
+    auto wait = [&](uint32_t bar, uint32_t parity) { ok = ok && mbar_wait_warp(bar, parity, abort_flag); };
+    auto wait_slot = [&]() {
+      wait(full + 8 * slot, use & 1);
+      if (++slot == SLOTS) { slot = 0; ++use; }
+    };
+    auto announce = [&]() { named_arrive(1 + (int)(event++ % EVENTS)); };
+    for (int k = 0; k < n_items && ok; ++k) {
+      const Item it(p, table, k, total);
+      const Keys keys(p, it.tile, it.z, p.parts);
+      if (keys.n == 0) continue;
+      for (int i = 0; i < keys.n + 2 && ok; ++i) {
+        if (i >= 2) {
+          const int J = jj + i - 2;
+          for (int s = 0; s < VP; ++s) wait_slot();
+          wait(bar_p + 8 * (J & 1), (uint32_t)(J >> 1) & 1);
+          announce();
+        }
+        if (i < keys.n) {
+          for (int s = 0; s < KP && ok; ++s) {
+            wait_slot();
+            announce();
+          }
+        }
+      }
+      if (++slot == SLOTS) { slot = 0; ++use; }  // the epilogue's slot
+      jj += keys.n;
+    }
   } else if (warp == ISSUER) {
     const bool el = elect_one();
     bool ok = true;
     int slot = 0, live = 0, jj = 0;  // jj: tiles of the items before
-    uint32_t use = 0;
-    uint32_t early = 0;  // whether the next slot was full when it was asked for, in front of the products of the one before it
-    auto wait_slot = [&]() {
-      ok = __all_sync(0xffffffffu, early != 0) || mbar_wait_warp(full + 8 * slot, use & 1, abort_flag);
-      if (ok) tc_fence_after();
-      return ok;
+    uint32_t event = 0;
+    // What the waiter has seen. The flag is read here, in front of the products, and asked behind them: an event that was announced
+    // after a wait had given up is the last, so that no other may be waited for
+    auto next_event = [&]() {
+      named_sync(1 + (int)(event++ % EVENTS));
+      ok = *abort_flag == 0;
+      tc_fence_after();
     };
-    auto ask_next = [&]() {
-      const bool wrap = slot + 1 == SLOTS;
-      early = mbar_test(full + 8 * (wrap ? 0 : slot + 1), (use + (wrap ? 1 : 0)) & 1);
-    };
-    auto advance = [&]() {
-      if (++slot == SLOTS) { slot = 0; ++use; }
-    };
+    auto advance = [&]() { slot = slot + 1 == SLOTS ? 0 : slot + 1; };
     for (int k = 0; k < n_items && ok; ++k) {
       const Item it(p, table, k, total);
       const Keys keys(p, it.tile, it.z, p.parts);
       if (keys.n == 0) continue;
       if (!(ok = mbar_wait_warp(bar_q, (uint32_t)live & 1, abort_flag))) break;
-      uint32_t early_p = 0;
       for (int i = 0; i < keys.n + 2 && ok; ++i) {
         if (i >= 2) {  // O += P[j] V[j]; P[j] lies over S[j]: 16 keys = 8 columns of bf16 pairs
           const int j = i - 2, J = jj + j;
-          if (!(ok = __all_sync(0xffffffffu, early_p != 0) || mbar_wait_warp(bar_p + 8 * (J & 1), (uint32_t)(J >> 1) & 1, abort_flag))) break;
+          next_event();  // V[j] and P[j]
           if (j == 0 && live > 0 && !(ok = mbar_wait_warp(bar_o_free, (uint32_t)(live - 1) & 1, abort_flag))) break;  // O of the item before has been read
-          tc_fence_after();
           const int valid = keys.valid(j, p, it.tile);
           constexpr uint32_t idesc = umma_idesc(128, HD, 1);
           const uint32_t pj = tmem + S_COL + (J & 1) * KT;
-          for (int s = 0; s < VP && wait_slot(); ++s) {
+          for (int s = 0; s < VP; ++s) {
             const int left = valid - s * KSUB;
             const uint64_t dv = umma_desc(ring + slot * SLOT, KSUB * 128, 1024);
             if (left >= KSUB) {
-              ask_next();
               if (el) {
 #pragma unroll
                 for (int x = 0; x < KSUB / 16; ++x) umma_f16_ts(tmem, pj + (s * (KSUB / 16) + x) * 8, dv + (uint64_t)(x * 128), idesc, (j | s | x) != 0 ? 1u : 0u);
@@ -407,7 +424,6 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
               }
-              ask_next();
               if (el) {
                 for (int x = 0; x < steps; ++x) umma_f16_ts(tmem, pj + (s * (KSUB / 16) + x) * 8, dv + (uint64_t)(x * 128), idesc, (j | s | x) != 0 ? 1u : 0u);
                 umma_commit_to(empty + 8 * slot);
@@ -421,15 +437,14 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             if (j + 1 == keys.n) umma_commit_to(bar_done);
           }
         }
-        early_p = 0;
         if (i < keys.n) {  // S[i]
           const int J = jj + i;
           const int valid = keys.valid(i, p, it.tile);
           const uint32_t d = tmem + S_COL + (J & 1) * KT;
           // a partial tile: the columns that hold a key, rounded up to the instruction's 16
           const uint32_t idesc = valid == KT ? umma_idesc(128, KT, 0) : umma_idesc(128, 0, 0) | ((uint32_t)((valid + 15) >> 4) << 18);
-          for (int s = 0; s < KP && wait_slot(); ++s) {
-            ask_next();
+          for (int s = 0; s < KP; ++s) {
+            next_event();
             if (el) {
 #pragma unroll
               for (int c = 0; c < SLABS; ++c) {
@@ -439,17 +454,17 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
               }
               umma_commit_to(empty + 8 * slot);
             }
-            if (i >= 1 && s + 1 == KP) early_p = mbar_test(bar_p + 8 * ((J - 1) & 1), (uint32_t)((J - 1) >> 1) & 1);
             advance();
+            if (!ok) break;
           }
-          if (ok && el) {
+          if (!ok) break;
+          if (el) {
             umma_commit_to(bar_s + 8 * (J & 1));
             if (i + 1 == keys.n) umma_commit_to(bar_q_free);
           }
         }
       }
       advance();  // the epilogue's slot
-      early = 0;
       jj += keys.n;
       ++live;
     }
