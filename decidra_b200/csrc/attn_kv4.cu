@@ -9,15 +9,16 @@
 // tile are (token, head) pairs, brought in by a 3-D TMA box. One CTA per SM goes through its items one after the other; the loads and
 // the first S products of an item run while the rows of the item before it are still being written. Keys come in tiles of 128, the
 // state's first, then the question's own:
-//   S = Q K^T      tcgen05.mma, both operands from shared memory, S[j] in one of two 128-column TMEM buffers
+//   S = Q K^T      tcgen05.mma, both operands from shared memory, S[j] in one of the 128-column TMEM buffers
 //   P = softmax    of S[j]: one thread per row and two groups of four warps, one for even, one for odd tiles. While one group is in its
 //                  exponentials the other is in the barriers, TMEM loads and stores around its own, so neither unit waits for a
 //                  round trip, and no row is split between threads. Rescaling is lazy: O is rescaled only when a row's maximum has
 //                  grown by more than 2^8; the groups hand the maximum in use from tile to tile through shared memory.
 //   O += P V       P as the TMEM operand (over S[j]), V from shared memory, O in TMEM
-// The tensor core runs S[0], S[1], then P.V[j], S[j + 2] in turn, so a tile's softmax has a whole tile's products to hide behind. (With
-// a second issuing warp S[j + 2] and P.V[j + 1] share the tensor core, and the loop S, softmax, P.V of a tile gets longer by that:
-// slower.) K and V come through one ring of 32 KB slots (16 KB at head_dim 64, a whole tile) in the order in which they are used, so that
+// The tensor core runs S[0], S[1], then P.V[j], S[j + 2] in turn, so a tile's softmax has a whole tile's products to hide behind; up to
+// head_dim 128 TMEM holds a third S, and a group finds its next scores there when it has written its weights (head_dim 128: 980 -> 885 ns
+// a tile, 64: 965 -> 800). One warp issues both products: S[j + 2] overwrites P[j], and only one thread's products are sure to run in
+// the order in which they were issued. K and V come through one ring of 32 KB slots (16 KB at head_dim 64, a whole tile) in the order in which they are used, so that
 // the loads run two and more product phases ahead. A barrier wait that is already satisfied still takes 100 to 170 cycles, which made
 // the issuing warp slower than the tensor core (2048 cycles a tile at head_dim 256: 4360 with 16 KB slots, 3080 with 32 KB), so another
 // warp waits in its place (364 -> 330 us over 64 questions of about 107 tokens and 2048 state rows).
@@ -43,7 +44,7 @@ using namespace tcc;
 constexpr int KT = 128;                   // keys of a tile
 constexpr int NUM_THREADS = 352, ISSUER = 8, LOADER = 9, WAITER = 10;  // warps 0-7: softmax and epilogue
 constexpr int MAX_ITEMS = 64;             // work items of a CTA
-constexpr uint32_t S_COL = 256;           // TMEM: O from column 0, S at 256 and 384
+constexpr int EVENTS = 14;                // hardware barriers 1 to 14
 constexpr float RESCALE = 8.0f;           // log2 units
 constexpr uint32_t BAR_BYTES = 512, ROW_BYTES = 4 * 128 * 4, TABLE_BYTES = MAX_ITEMS * 8;
 
@@ -55,8 +56,12 @@ template <int HD> struct Shape {
   static constexpr uint32_t Q_BYTES = 128 * HD * 2;
   static constexpr int SLOTS = HD == 256 ? 5 : HD == 128 ? 6 : 10;
   static constexpr int KP = NKB / SLABS, VP = KT / KSUB;      // slots of a tile's K and V
+  // TMEM: O from column 0, the S buffers behind it
+  static constexpr int SB = HD == 256 ? 2 : 3;
+  static constexpr uint32_t S_COL = HD == 256 ? 256 : 128;
   static constexpr uint32_t SMEM = Q_BYTES + SLOTS * SLOT + ROW_BYTES + BAR_BYTES + TABLE_BYTES;
   static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
+  static_assert(SLOTS + SB < EVENTS, "events announced ahead");
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -151,7 +156,6 @@ struct Keys {
   }
 };
 
-constexpr int EVENTS = 14;  // hardware barriers 1 to 14
 __device__ __forceinline__ void named_sync(int id) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory"); }
 __device__ __forceinline__ void named_arrive(int id) { asm volatile("barrier.cta.arrive %0, 64;" ::"r"(id) : "memory"); }
 
@@ -167,17 +171,31 @@ __device__ __forceinline__ void st_global_if(void* p, uint2 v, bool there) {
   asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %3, 0;\n@q st.global.v2.b32 [%0], {%1, %2};\n}" ::"l"(p), "r"(v.x), "r"(v.y), "r"((int)there) : "memory");
 }
 
+// A causal prompt's late tiles are its longest and go first: sorted by where in their prompts they are, or, with more prompts than the
+// lanes of a warp hold (by then a CTA has many items) or the keys split, from the batch's end. Sorted items go there and back again
+// through the CTAs, so that the CTAs' sums stay close. Five prompts of 1051 to 1814 tokens, 16 heads of 128 over 2 K/V heads: from the
+// end 91 to 94 us (the busiest SM has 58 key tiles, the mean is 43), sorted 72 to 83.
+constexpr int SORTED = 4;  // prompts per lane
+__device__ __forceinline__ bool sorted_items(const Params& p) { return p.causal && p.parts == 1 && p.B <= SORTED * 32; }
+// The k-th item of a CTA. All in one direction otherwise: CTAs next to each other then stay closer in time and in what they read
+// (64 questions, there and back: 338 us, one way 333).
+__device__ __forceinline__ int item_of(const Params& p, int k) {
+  const int c = (int)blockIdx.x, n = (int)gridDim.x;
+  return k * n + (sorted_items(p) && (k & 1) ? n - 1 - c : c);
+}
+// The tile at place ti of the unsorted order
+__device__ __forceinline__ int tile_of(const Params& p, int ti, int total) { return p.causal ? total - 1 - ti : ti; }
+
 // What a work item is: its tokens, heads, part and keys. Every role goes through the same items; n_tiles == 0 (more parts than key tiles)
 // leaves one out.
 struct Item {
   Tile tile;
   int hg, kh, head0, z, ti;
   __device__ __forceinline__ Item(const Params& p, const int2* table, int k, int total) {
-    const int nh = p.kv * p.sub, w = (int)blockIdx.x + k * (int)gridDim.x, rest = w / nh;
+    const int nh = p.kv * p.sub, w = item_of(p, k), rest = w / nh;
     hg = w - rest * nh;
     z = rest / total;
-    ti = rest - z * total;
-    if (p.causal) ti = total - 1 - ti;  // a causal prompt's late tiles are its longest: they start first
+    ti = tile_of(p, rest - z * total, total);
     // uniform for the compiler too, so that what the issuing warps compute from it stays on the uniform datapath
     const int b = __shfl_sync(0xffffffffu, table[k].x, 0);
     tile.t0 = __shfl_sync(0xffffffffu, table[k].y, 0);
@@ -194,8 +212,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKs, const __grid_constant__ CUtensorMap tmVs,
                      const __grid_constant__ CUtensorMap tmKo, const __grid_constant__ CUtensorMap tmVo, const Params p) {
   using D = Shape<HD>;
-  constexpr int NKB = D::NKB, SLABS = D::SLABS, KSUB = D::KSUB, SLOTS = D::SLOTS, KP = D::KP, VP = D::VP;
-  constexpr uint32_t SLOT = D::SLOT;
+  constexpr int NKB = D::NKB, SLABS = D::SLABS, KSUB = D::KSUB, SLOTS = D::SLOTS, KP = D::KP, VP = D::VP, SB = D::SB;
+  constexpr uint32_t SLOT = D::SLOT, S_COL = D::S_COL;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t q_base = smem_u32(smem), ring = q_base + D::Q_BYTES;
   float* m_used = reinterpret_cast<float*>(smem + D::Q_BYTES + SLOTS * SLOT);  // [2][128] by tile parity
@@ -203,14 +221,15 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   uint8_t* bars_ptr = smem + D::Q_BYTES + SLOTS * SLOT + ROW_BYTES;
   int2* table = reinterpret_cast<int2*>(bars_ptr + BAR_BYTES);                 // (sequence, first token) of the CTA's items
   const uint32_t bars = ring + SLOTS * SLOT + ROW_BYTES;
-  // by tile parity: S done, P written, P.V done, maximum published. Tiles are counted through all items of the CTA. A parity wait is
-  // sound while the barrier is at most one phase behind the waiter: with two barriers that is two tiles, and nobody runs two tiles
-  // ahead of P.V (S[j] comes behind P.V[j - 2]). Once per item: Q loaded, Q no longer needed, last P.V done, sums exchanged, O read, the
+  // by S buffer: S done, P written; by tile parity: P.V done, maximum published. Tiles are counted through all items of the CTA. A
+  // parity wait is sound while the barrier is at most one phase behind the waiter: S[j + SB] comes behind P.V[j], P[j + SB] behind that,
+  // and a tile's weights are written only after the maximum of the tile before it was read and that tile's P.V, if asked for, seen.
+  // Once per item: Q loaded, Q no longer needed, last P.V done, sums exchanged, O read, the
   // epilogue's slot free.
-  const uint32_t bar_s = bars, bar_p = bars + 16, bar_o = bars + 32, bar_m = bars + 48;
-  const uint32_t bar_q = bars + 64, bar_q_free = bars + 72, bar_done = bars + 80, bar_l = bars + 88, bar_o_free = bars + 96, bar_e = bars + 104;
-  const uint32_t full = bars + 112, empty = full + 8 * SLOTS;
-  static_assert(112 + 16 * SLOTS + 64 <= BAR_BYTES, "barrier area");
+  const uint32_t bar_s = bars, bar_p = bars + 24, bar_o = bars + 48, bar_m = bars + 64;
+  const uint32_t bar_q = bars + 80, bar_q_free = bars + 88, bar_done = bars + 96, bar_l = bars + 104, bar_o_free = bars + 112, bar_e = bars + 120;
+  const uint32_t full = bars + 128, empty = full + 8 * SLOTS;
+  static_assert(128 + 16 * SLOTS + 64 <= BAR_BYTES, "barrier area");
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars_ptr + BAR_BYTES - 64);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars_ptr + BAR_BYTES - 60);
   int* sums = reinterpret_cast<int*>(bars_ptr + BAR_BYTES - 56);
@@ -221,9 +240,11 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     return;
   }
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < SB; ++i) {
       mbar_init(bar_s + 8 * i, 1);
       mbar_init(bar_p + 8 * i, 128);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(bar_o + 8 * i, 1);
       mbar_init(bar_m + 8 * i, 128);
     }
@@ -258,17 +279,47 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   int total = scan_tiles(p, sums, [](int, int, int) {});
   total = __shfl_sync(0xffffffffu, total, 0);
   const int nh = p.kv * p.sub, all_items = total * nh * p.parts;
-  const int n_items = min(MAX_ITEMS, ((int)blockIdx.x < all_items ? (all_items - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0));
-  int* wanted = reinterpret_cast<int*>(l_part);  // the items' tile numbers; the rows' sums come here later
-  if ((int)threadIdx.x < n_items) {
-    const int ti = ((int)blockIdx.x + (int)threadIdx.x * (int)gridDim.x) / nh % total;
-    wanted[threadIdx.x] = p.causal ? total - 1 - ti : ti;
+  int n_items = all_items / (int)gridDim.x;
+  if (item_of(p, n_items) < all_items) ++n_items;
+  n_items = min(MAX_ITEMS, n_items);
+  if (sorted_items(p)) {
+    int n[SORTED];
+#pragma unroll
+    for (int q = 0; q < SORTED; ++q) {
+      int off, len;
+      n[q] = q * 32 + lane < p.B ? tiles_of(p, q * 32 + lane, off, len) : 0;
+    }
+    auto behind = [&](int i) {  // tiles with at least i others of their prompt in front of them
+      int c = 0;
+#pragma unroll
+      for (int q = 0; q < SORTED; ++q) c += max(0, n[q] - i);
+      return __reduce_add_sync(0xffffffffu, c);
+    };
+    for (int k = warp; k < n_items; k += NUM_THREADS / 32) {
+      const int place = item_of(p, k) / nh;
+      int i = 0, not_i = total;  // behind(i) > place >= behind(not_i)
+      while (not_i - i > 1) {
+        const int mid = (i + not_i) >> 1;
+        if (behind(mid) > place) i = mid;
+        else not_i = mid;
+      }
+      int before = place - behind(i + 1);  // prompts with such a tile in front of the one that is meant
+#pragma unroll
+      for (int q = 0; q < SORTED; ++q) {
+        const uint32_t have = __ballot_sync(0xffffffffu, n[q] > i);
+        if (n[q] > i && __popc(have & ((1u << lane) - 1u)) == before) table[k] = make_int2(q * 32 + lane, i * p.tokens);
+        before -= __popc(have);
+      }
+    }
+  } else {
+    int* wanted = reinterpret_cast<int*>(l_part);  // the items' tile numbers; the rows' sums come here later
+    if ((int)threadIdx.x < n_items) wanted[threadIdx.x] = tile_of(p, item_of(p, (int)threadIdx.x) / nh % total, total);
+    __syncthreads();
+    scan_tiles(p, sums, [&](int b, int before, int n) {
+      for (int k = 0; k < n_items; ++k)
+        if (wanted[k] >= before && wanted[k] < before + n) table[k] = make_int2(b, (wanted[k] - before) * p.tokens);
+    });
   }
-  __syncthreads();
-  scan_tiles(p, sums, [&](int b, int before, int n) {
-    for (int k = 0; k < n_items; ++k)
-      if (wanted[k] >= before && wanted[k] < before + n) table[k] = make_int2(b, (wanted[k] - before) * p.tokens);
-  });
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -303,10 +354,10 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
         for (int c = 0; c < NKB; ++c) tma_load_3d(q_base + c * 16384, &tmQ, bar_q, c * 64, it.head0, it.tile.off + it.tile.t0);
       }
-      for (int i = 0; i < keys.n + 2 && ok; ++i) {
-        if (i >= 2) {
-          const bool st = keys.state(i - 2);
-          const int row = keys.key0(i - 2) + (st ? 0 : it.tile.off);
+      for (int i = 0; i < keys.n + SB && ok; ++i) {
+        if (i >= SB) {
+          const bool st = keys.state(i - SB);
+          const int row = keys.key0(i - SB) + (st ? 0 : it.tile.off);
           for (int s = 0; s < VP && next_slot(); ++s) {
             if (el) {
               mbar_expect_tx(full + 8 * slot, SLOT);
@@ -346,11 +397,11 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     // ---- waits for the issuer: the same barriers in the same order, each handed on through a hardware barrier. A satisfied mbarrier wait
     // takes 100 to 170 cycles, the hardware barrier 20 to 30; the tensor core's queue holds two or three products, so that what the
     // issuing warp waits is lost. V's slots are waited for in front of P, which comes last, and share its event. At most the ring's
-    // slots and two P are announced ahead, fewer than there are EVENTS. A wait that gave up is still announced, with the flag up, and
+    // slots and SB P are announced ahead, fewer than there are EVENTS. A wait that gave up is still announced, with the flag up, and
     // nothing after it ----------------------------------------------------------------------------------------------------------
     bool ok = true;
-    int slot = 0, jj = 0;
-    uint32_t use = 0, event = 0;
+    int slot = 0, pb = 0;
+    uint32_t use = 0, event = 0, pp = 0;  // pb, pp: buffer and phase of the next P
     auto wait = [&](uint32_t bar, uint32_t parity) { ok = ok && mbar_wait_warp(bar, parity, abort_flag); };
     auto wait_slot = [&]() {
       wait(full + 8 * slot, use & 1);
@@ -361,11 +412,11 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       const Item it(p, table, k, total);
       const Keys keys(p, it.tile, it.z, p.parts);
       if (keys.n == 0) continue;
-      for (int i = 0; i < keys.n + 2 && ok; ++i) {
-        if (i >= 2) {
-          const int J = jj + i - 2;
+      for (int i = 0; i < keys.n + SB && ok; ++i) {
+        if (i >= SB) {
           for (int s = 0; s < VP; ++s) wait_slot();
-          wait(bar_p + 8 * (J & 1), (uint32_t)(J >> 1) & 1);
+          wait(bar_p + 8 * pb, pp);
+          if (++pb == SB) { pb = 0; pp ^= 1; }
           announce();
         }
         if (i < keys.n) {
@@ -376,12 +427,11 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         }
       }
       if (++slot == SLOTS) { slot = 0; ++use; }  // the epilogue's slot
-      jj += keys.n;
     }
   } else if (warp == ISSUER) {
     const bool el = elect_one();
     bool ok = true;
-    int slot = 0, live = 0, jj = 0;  // jj: tiles of the items before
+    int slot = 0, live = 0, jj = 0, sb = 0, pb = 0;  // jj: tiles of the items before; sb, pb: buffers of the next S and P
     uint32_t event = 0;
     // What the waiter has seen. The flag is read here, in front of the products, and asked behind them: an event that was announced
     // after a wait had given up is the last, so that no other may be waited for
@@ -396,14 +446,15 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       const Keys keys(p, it.tile, it.z, p.parts);
       if (keys.n == 0) continue;
       if (!(ok = mbar_wait_warp(bar_q, (uint32_t)live & 1, abort_flag))) break;
-      for (int i = 0; i < keys.n + 2 && ok; ++i) {
-        if (i >= 2) {  // O += P[j] V[j]; P[j] lies over S[j]: 16 keys = 8 columns of bf16 pairs
-          const int j = i - 2, J = jj + j;
+      for (int i = 0; i < keys.n + SB && ok; ++i) {
+        if (i >= SB) {  // O += P[j] V[j]; P[j] lies over S[j]: 16 keys = 8 columns of bf16 pairs
+          const int j = i - SB, J = jj + j;
           next_event();  // V[j] and P[j]
           if (j == 0 && live > 0 && !(ok = mbar_wait_warp(bar_o_free, (uint32_t)(live - 1) & 1, abort_flag))) break;  // O of the item before has been read
           const int valid = keys.valid(j, p, it.tile);
           constexpr uint32_t idesc = umma_idesc(128, HD, 1);
-          const uint32_t pj = tmem + S_COL + (J & 1) * KT;
+          const uint32_t pj = tmem + S_COL + pb * KT;
+          pb = pb + 1 == SB ? 0 : pb + 1;
           for (int s = 0; s < VP; ++s) {
             const int left = valid - s * KSUB;
             const uint64_t dv = umma_desc(ring + slot * SLOT, KSUB * 128, 1024);
@@ -438,9 +489,9 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           }
         }
         if (i < keys.n) {  // S[i]
-          const int J = jj + i;
           const int valid = keys.valid(i, p, it.tile);
-          const uint32_t d = tmem + S_COL + (J & 1) * KT;
+          const uint32_t d = tmem + S_COL + sb * KT, done = bar_s + 8 * sb;
+          sb = sb + 1 == SB ? 0 : sb + 1;
           // a partial tile: the columns that hold a key, rounded up to the instruction's 16
           const uint32_t idesc = valid == KT ? umma_idesc(128, KT, 0) : umma_idesc(128, 0, 0) | ((uint32_t)((valid + 15) >> 4) << 18);
           for (int s = 0; s < KP; ++s) {
@@ -459,7 +510,7 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           }
           if (!ok) break;
           if (el) {
-            umma_commit_to(bar_s + 8 * (J & 1));
+            umma_commit_to(done);
             if (i + 1 == keys.n) umma_commit_to(bar_q_free);
           }
         }
@@ -472,7 +523,7 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     // ---- softmax: group h takes the tiles of its parity; thread r of a group has row r ----------------------------------------------
     const int h = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_tmem = tmem + lanes + S_COL + h * KT;
+    const uint32_t s_tmem0 = tmem + lanes + S_COL;
     const int tt = r / G;  // the row's token in the tile
     bool ok = true;
     int live = 0, jj = 0;
@@ -495,7 +546,8 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     }
     float m = -INFINITY, l = 0.f;  // what this group's part of the denominator is relative to, and that part
     for (int j = (h ^ jj) & 1; j < n_tiles && ok; j += 2) {
-      const uint32_t ph = (uint32_t)((jj + j) >> 1) & 1, ph_before = (uint32_t)((jj + j - 1) >> 1) & 1;
+      const uint32_t J = (uint32_t)(jj + j), ph_before = ((J - 1) >> 1) & 1, b = SB == 2 ? (uint32_t)h : J % SB;
+      const uint32_t s_tmem = s_tmem0 + b * KT;
       int lim = keys.valid(j, p, tile);
       if (p.causal && !keys.state(j)) lim = min(lim, tok + 1 - keys.key0(j));
       // the maximum in use so far, from the other group's tile before this one: published long before S[j] is there
@@ -505,7 +557,7 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         if (!ok) break;
         before = m_used[(h ^ 1) * 128 + r];
       }
-      ok = __all_sync(0xffffffffu, mbar_wait(bar_s + 8 * h, ph, abort_flag));
+      ok = __all_sync(0xffffffffu, mbar_wait(bar_s + 8 * b, SB == 2 ? (J >> 1) & 1 : (J / SB) & 1, abort_flag));
       if (!ok) break;
       tc_fence_after();
       // The scores are read from TMEM twice, 64 at a time, once for the maximum and once for the weights: a thread that keeps all 128 has
@@ -575,7 +627,7 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(bar_p + 8 * h);
+      mbar_arrive(bar_p + 8 * b);
     }
     // ---- epilogue: either group takes half of the head's dimensions, each warp its 32 rows, CH dimensions at a time: from TMEM (lane =
     // row) to the warp's part of the epilogue's slot, and from there in whole rows ---------------------------------------------------
