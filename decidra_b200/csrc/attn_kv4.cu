@@ -563,15 +563,16 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       // The scores are read from TMEM twice, 64 at a time, once for the maximum and once for the weights: a thread that keeps all 128 has
       // none of its registers left, and the straight code for them evicts the issuing warp's from the instruction cache (419 -> 364 us
       // over 64 questions of about 107 tokens and 2048 keys).
-      const bool partial = __any_sync(0xffffffffu, lim < KT);
+      // Keys that no row of the warp sees are left out 64 at a time, and only where some row sees some are they masked one by one.
+      const int all_see = __reduce_min_sync(0xffffffffu, lim), some_see = __reduce_max_sync(0xffffffffu, lim);
       float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-      for (int c = 0; c < KT; c += 64) {
+      for (int c = 0; c < KT && c < some_see; c += 64) {
         float x[64];
 #pragma unroll
         for (int i = 0; i < 64; i += 32) tmem_ld32(s_tmem + c + i, reinterpret_cast<uint32_t*>(x + i));
         tmem_ld_wait();
-        if (partial) {
+        if (all_see < c + 64) {
 #pragma unroll
           for (int i = 0; i < 64; ++i) x[i] = c + i < lim ? x[i] : -INFINITY;
         }
@@ -606,15 +607,21 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       float l4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
       for (int c = 0; c < KT; c += 64) {
+        uint32_t w[32];
+        if (c >= some_see) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) w[i] = 0u;
+          tmem_st32(s_tmem + c / 2, w);
+          continue;
+        }
         float x[64];
 #pragma unroll
         for (int i = 0; i < 64; i += 32) tmem_ld32(s_tmem + c + i, reinterpret_cast<uint32_t*>(x + i));
         tmem_ld_wait();
-        if (partial) {
+        if (all_see < c + 64) {
 #pragma unroll
           for (int i = 0; i < 64; ++i) x[i] = c + i < lim ? x[i] : -INFINITY;
         }
-        uint32_t w[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           const float a = ex2(fmaf(x[2 * i], p.scale_log2e, neg)), b = ex2(fmaf(x[2 * i + 1], p.scale_log2e, neg));
