@@ -110,30 +110,36 @@ __device__ __forceinline__ int tiles_of(const Params& p, int i, int& off, int& l
 }
 
 // Calls found(sequence, its tiles before it, its tiles) for every sequence, each in one thread of the block, and returns the number of
-// all tiles. `sums` holds an int per warp.
+// all tiles. `sums` holds an int per warp. Offsets that rise have at most max_tiles; where others add up to more, the sums stay at
+// max_tiles + 1 (so that they cannot overflow), and the batch counts as empty.
 template <typename F>
 __device__ __forceinline__ int scan_tiles(const Params& p, int* sums, F found) {
-  const int nt = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = nt >> 5;
+  const int nt = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = nt >> 5, most = p.max_tiles + 1;
   int base = 0;
   for (int b0 = 0; b0 < p.B; b0 += nt) {
     const int i = b0 + (int)threadIdx.x;
     int off, len;
-    const int n = i < p.B ? tiles_of(p, i, off, len) : 0;
+    const int n = i < p.B ? min(tiles_of(p, i, off, len), most) : 0;
     int incl = n;
     for (int o = 1; o < 32; o <<= 1) {
       const int x = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += x;
+      if (lane >= o) incl = min(incl + x, most);
     }
     if (lane == 31) sums[warp] = incl;
+    const int up = __shfl_up_sync(0xffffffffu, incl, 1);
     __syncthreads();
     int before = base, all = base;
     for (int w = 0; w < nw; ++w) {
-      if (w < warp) before += sums[w];
-      all += sums[w];
+      if (w < warp) before = min(before + sums[w], most);
+      all = min(all + sums[w], most);
     }
     __syncthreads();
-    if (n > 0) found(i, before + incl - n, n);
+    if (n > 0) found(i, lane > 0 ? min(before + up, most) : before, n);
     base = all;
+  }
+  if (base > p.max_tiles) {
+    set_err(p.err, DERR_OFFSETS);
+    return 0;
   }
   return base;
 }
@@ -752,7 +758,7 @@ __global__ void __launch_bounds__(128) kv4_attention_merge_kernel(const Params p
   __shared__ int sums[4], found[3];
   if (threadIdx.x == 0) found[0] = -1;
   __syncthreads();
-  scan_tiles(p, sums, [&](int b, int before, int n) {
+  const int all = scan_tiles(p, sums, [&](int b, int before, int n) {
     const int ti = blockIdx.x;
     if (ti < before || ti >= before + n) return;
     int off, len;
@@ -763,7 +769,7 @@ __global__ void __launch_bounds__(128) kv4_attention_merge_kernel(const Params p
   });
   __syncthreads();
   const int lane = threadIdx.x & 31, r = blockIdx.z * 4 + (threadIdx.x >> 5), G = p.G;
-  if (found[0] < 0 || r >= found[2] * G) return;
+  if (all == 0 || found[0] < 0 || r >= found[2] * G) return;
   const int hg = blockIdx.y, kh = hg / p.sub, tt = r / G;
   const int head = kh * (p.heads / p.kv) + (hg - kh * p.sub) * G + r - tt * G;
   const size_t step = (size_t)gridDim.y * gridDim.x * 128, row0 = ((size_t)hg * gridDim.x + blockIdx.x) * 128 + r;
@@ -813,7 +819,8 @@ int sm_count() {
 }
 
 struct Plan {
-  int G, sub, tokens, tiles, parts;
+  int G, sub, tokens, parts;
+  long long tiles;
   size_t state_bytes, ml_bytes, o_bytes;
 };
 Plan plan_of(int B, int T, int n_state, int heads, int kv, int hd) {
@@ -823,12 +830,13 @@ Plan plan_of(int B, int T, int n_state, int heads, int kv, int hd) {
   while (p.G > 128 || group % p.G != 0) --p.G;  // the rows of one token fit a tile
   p.sub = group / p.G;
   p.tokens = 128 / p.G;
-  p.tiles = (T + p.tokens - 1) / p.tokens + B;
+  p.tiles = (long long)(T + p.tokens - 1LL) / p.tokens + B;
   // split the keys where there is no CTA for every SM and the state is at least eight tiles long: about two CTAs per SM, at least
   // two key tiles per part
-  const int ctas = p.tiles * kv * p.sub, st_tiles = (n_state + KT - 1) / KT, sms = sm_count();
+  const long long ctas = p.tiles * kv * p.sub;
+  const int st_tiles = (int)((n_state + KT - 1LL) / KT), sms = sm_count();
   p.parts = 1;
-  if (ctas <= sms && st_tiles >= 8) p.parts = max(1, min(min(2 * sms / ctas, st_tiles / 2), 128));
+  if (ctas <= sms && st_tiles >= 8) p.parts = max(1, min(min(2 * sms / (int)ctas, st_tiles / 2), 128));
   p.state_bytes = (size_t)2 * n_state * kv * hd * 2;
   const size_t rows = p.parts > 1 ? (size_t)p.parts * ctas * 128 : 0;
   p.ml_bytes = rows * sizeof(float2);
@@ -857,7 +865,7 @@ cudaError_t run(const Kv4QuestionArgs& a, const Plan& pl, uint8_t* ws, cudaStrea
   p.scale_log2e = (1.0f / sqrtf((float)HD)) * 1.4426950408889634f;
   p.err = a.err;
   p.parts = pl.parts;
-  p.max_tiles = pl.tiles;
+  p.max_tiles = (int)pl.tiles;
   p.ws_ml = (float2*)(ws + pl.state_bytes);
   p.ws_o = (float*)(ws + pl.state_bytes + pl.ml_bytes);
   const uint64_t width = (uint64_t)a.kv * HD;
@@ -877,13 +885,13 @@ cudaError_t run(const Kv4QuestionArgs& a, const Plan& pl, uint8_t* ws, cudaStrea
   if (a.n_state > 0) CUDA_TRY(launch_kv4_read<bf16>(a.state, a.n_state, nullptr, ks, vs, a.n_state, a.kv, HD, nullptr, s));
   CUDA_TRY(cudaFuncSetAttribute(kv4_attention_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<HD>::SMEM));
   // one CTA per SM, more only where one would have more items than its table holds
-  const long long items = (long long)pl.tiles * a.kv * pl.sub * pl.parts;
+  const long long items = pl.tiles * a.kv * pl.sub * pl.parts;
   if (items > (1 << 30)) return cudaErrorInvalidValue;
   const unsigned grid = (unsigned)max(min(items, (long long)sm_count()), (items + MAX_ITEMS - 1) / MAX_ITEMS);
   auto map = [](const TcTensorMap& m) -> const CUtensorMap& { return *reinterpret_cast<const CUtensorMap*>(&m); };
   kv4_attention_kernel<HD><<<grid, NUM_THREADS, Shape<HD>::SMEM, s>>>(map(q), map(ksm), map(vsm), map(ko), map(vo), p);
   CUDA_TRY(cudaGetLastError());
-  if (pl.parts > 1) kv4_attention_merge_kernel<HD><<<dim3(pl.tiles, a.kv * pl.sub, 32), 128, 0, s>>>(p, pl.parts);
+  if (pl.parts > 1) kv4_attention_merge_kernel<HD><<<dim3((unsigned)pl.tiles, a.kv * pl.sub, 32), 128, 0, s>>>(p, pl.parts);
   return cudaGetLastError();
 }
 

@@ -7,9 +7,9 @@
 // blocks in turn), so that a CTA reads whole rows of the cache: one head's 128 bytes of every 512, and 16 of every 64 bytes of scales,
 // cost 17 % more DRAM traffic than they hold. Each warp has room for one block of its own in shared memory (cp.async, no barrier between
 // warps): the next K is on its way from the end of the S products on, the next V from the end of the P.V products, so that half a block
-// per warp is always in flight and twelve warps fit on an SM (with two and three whole blocks a warp and eight warps, two thirds of
-// the issue slots stayed empty). Few query rows share each key (tokens x heads of the group, eight per MMA column tile), so the kernel lives on getting
-// 0.5625 bytes a value from HBM into matrix fragments:
+// per warp is always in flight and twelve warps fit on an SM (two and three whole blocks a warp and eight warps: 162 us where this takes
+// 149, half of the issue slots empty). Few query rows share each key (tokens x heads of the group, eight per MMA column tile), so the
+// kernel lives on getting 0.5625 bytes a value from HBM into matrix fragments:
 //   S^T[16 keys, 8 rows]  += K[16 keys, 16 dims] Q^T      mma.m16n8k16 with the KEYS as the 16-row operand: all of it is used
 //   O^T[16 dims, 8 rows]  += V^T[16 dims, 16 keys] P^T    even for one token of six heads, where rows as M would fill 6 of 16
 // The fragments are made in registers straight from the code words. The order of the contracted dimensions is free as long as Q has
@@ -120,11 +120,10 @@ struct Sequence {
 __device__ __forceinline__ Sequence sequence(const Kv4DecodeArgs& a, int b, bool report) {
   Sequence s;
   s.off = a.cu[b];
-  s.L = a.cu[b + 1] - s.off;
-  if (s.off < 0 || s.L < 0 || s.L > a.T - s.off) {
-    if (report) set_err(a.err, DERR_OFFSETS);
-    s.L = 0;
-  }
+  const int stop = a.cu[b + 1];
+  const bool sound = s.off >= 0 && stop >= s.off && stop <= a.T;  // compared before they are subtracted: the difference of bad ones may overflow
+  s.L = sound ? stop - s.off : 0;
+  if (!sound && report) set_err(a.err, DERR_OFFSETS);
   const int64_t st = a.seg_start[b];
   s.len = a.seg_len[b];
   s.start = (size_t)st;
@@ -695,7 +694,8 @@ Plan plan_of(int B, int kv, int max_len) {
   p.hc = kv % 4 == 0 ? 4 : kv % 2 == 0 ? 2 : 1;
   p.sms = sm_count();
   const long long blocks = max(1LL, ((long long)max_len + KB - 1) / KB);
-  p.q_min = (int)max(2LL * WARPS / p.hc, ((long long)B * (kv / p.hc) * blocks / (2 * p.sms) + 3) / 4);
+  const double share = (double)B * (kv / p.hc) * (double)blocks / (8.0 * p.sms);  // an eighth of what the CTAs of two per SM would take
+  p.q_min = (int)max(2LL * WARPS / p.hc, (long long)min(ceil(share), (double)blocks));
   p.max_parts = (int)((blocks + p.q_min - 1) / p.q_min) + 1;
   return p;
 }
@@ -734,7 +734,8 @@ cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, void* workspace, cudaStrea
   p.ws_ml = (float2*)(p.ws_o + parts * a.hd);
   p.ws_n = (int*)(p.ws_ml + parts);
   // column tiles of eight rows by the rows of a sequence of average length; longer ones take several rounds over their keys
-  const int rows = ((a.T + a.B - 1) / a.B) * (a.heads / a.kv), n = plan.sms;
+  const long long rows = ((long long)a.T + a.B - 1) / a.B * (a.heads / a.kv);
+  const int n = plan.sms;
   if (a.hd == 256) return rows <= 8 ? kvd::run<256, 1>(p, n, s) : kvd::run<256, 2>(p, n, s);
   if (a.hd == 128) return rows <= 8 ? kvd::run<128, 1>(p, n, s) : rows <= 16 ? kvd::run<128, 2>(p, n, s) : kvd::run<128, 4>(p, n, s);
   return rows <= 8 ? kvd::run<64, 1>(p, n, s) : rows <= 16 ? kvd::run<64, 2>(p, n, s) : kvd::run<64, 4>(p, n, s);

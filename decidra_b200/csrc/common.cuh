@@ -16,8 +16,8 @@ enum : int {
   DERR_ATTN_TIMEOUT = 4,
   DERR_POSITION_RANGE = 5, // RoPE position beyond the table
   DERR_GDN_TIMEOUT = 6,
-  DERR_OFFSETS = 8,       // packed offsets that fall or leave the batch
-  DERR_CACHE_ROW = 7      // a row of a 4-bit K/V cache, or a stretch of rows, outside the cache
+  DERR_CACHE_ROW = 7,     // a row of a 4-bit K/V cache, or a stretch of rows, outside the cache
+  DERR_OFFSETS = 8        // packed offsets that fall or leave the batch
 };
 
 __device__ __forceinline__ void set_err(int* err, int code) {

@@ -685,9 +685,11 @@ DCD_API int dcd_k_kv4_read(const void* k_codes, const void* k_scales, const void
  * of them, or with causal != 0 those up to itself), out = softmax(q k / sqrt(hd)) v, times sigmoid(gate) where gate_qg (laid out as
  * there) is given. n_state 0 with causal 1 is causal attention over packed prompts; the cache pointers may then be NULL. bf16; any
  * heads that kv divides; hd 64, 128 or 256; q [T, heads, hd], k_own and v_own [T, kv, hd] with row strides in elements, multiples of 8,
- * 16-byte aligned, qg_stride at most 2^24; out [T, heads, hd]. cu_seqlens [B + 1] rises from 0 to at most T; rows of out behind the last sequence
- * are left as they were. workspace: dcd_k_attention_kv4_workspace bytes (0: none is needed), 16-byte aligned, not shared by calls that
- * may overlap. */
+ * 16-byte aligned, qg_stride at most 2^24; out [T, heads, hd]. cu_seqlens [B + 1] rises from 0 to at most T; a sequence whose offsets
+ * fall or leave [0, T] sets *err and is left out, and rows of out that no sequence has, those behind the last one too, are left as they
+ * were. A NaN or an infinity in a question's values may reach all of that question's tokens, later ones' under causal too (its weight
+ * there is 0, and 0 times it is NaN), and nothing outside the question. workspace: dcd_k_attention_kv4_workspace bytes (0: none is
+ * needed), 16-byte aligned, not shared by calls that may overlap. */
 DCD_API size_t dcd_k_attention_kv4_workspace(int B, int T, int n_state, int heads, int kv, int hd);
 DCD_API int dcd_k_attention_kv4(const void* q, size_t q_stride, const void* k_own, size_t k_stride, const void* v_own, size_t v_stride, const void* k_codes,
                                 const void* k_scales, const void* v_codes, const void* v_scales, int n_state, const void* gate_qg, size_t qg_stride,
@@ -695,8 +697,9 @@ DCD_API int dcd_k_attention_kv4(const void* q, size_t q_stride, const void* k_ow
                                 size_t workspace_bytes, int* err, void* stream);
 /* The form for new tokens: sequence b's rows in the cache are [seg_start[b], seg_start[b] + seg_len[b]), its packed tokens
  * [cu_seqlens[b], cu_seqlens[b + 1]) are the newest ones, already written there: the last token sees every row of the stretch, each
- * one before it a row less. Stretches may be shared or overlap. A token that sees no row (more tokens than rows) gives 0. A stretch that leaves the cache or is longer
- * than max_len sets *err, and its tokens give 0. max_len is at most 2^30. Meant for one to a few tokens a sequence; every other operand as above. */
+ * one before it a row less. Stretches may be shared or overlap. A token that sees no row (more tokens than rows) gives 0. A stretch
+ * that leaves the cache or is longer than max_len sets *err, and its tokens give 0. max_len is at most 2^30 (the workspace grows with
+ * it). Meant for one to a few tokens a sequence; every other operand as above. */
 DCD_API size_t dcd_k_attention_kv4_decode_workspace(int B, int T, int max_len, int heads, int kv, int hd);
 DCD_API int dcd_k_attention_kv4_decode(const void* q, size_t q_stride, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
                                        size_t cache_rows, const int64_t* seg_start, const int32_t* seg_len, int max_len, const void* gate_qg,

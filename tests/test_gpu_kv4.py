@@ -499,6 +499,99 @@ def test_attention_offsets_beyond_32_bits(G):
     close(d.out[:1], want, spread)
 
 
+@pytest.mark.parametrize("lens", [[(7 * i) % 45 for i in range(40)], [(5 * i) % 23 for i in range(131)], [1] * 33])
+@pytest.mark.parametrize("heads,kv,hd,S", [(16, 2, 128, 0), (24, 4, 256, 140), (8, 8, 64, 3)])
+def test_attention_causal_prompts_by_the_dozen(G, heads, kv, hd, S, lens):
+    """More prompts than a warp has lanes, and more than its lanes hold: the order of the work changes, not the result."""
+    c = Questions(lens, S, heads, kv, hd, True, False)
+    c.launch(G)
+    c.check()
+
+
+@pytest.mark.parametrize("causal,lens", [(True, [1 + (37 * i) % 200 for i in range(100)]), (False, [1 + i % 3 for i in range(200)])])
+def test_attention_more_items_than_one_wave_lists(G, causal, lens):
+    """64 K/V heads, a query head each: about ten thousand work items."""
+    c = Questions(lens, 0, 64, 64, 64, causal, False)
+    c.launch(G)
+    c.check()
+
+
+BAD_OFFSETS = [([0, 5, 3, 12], [0]), ([-1, 4, 9, 12], [1, 2]), ([0, 4, 99, 12], [0]), ([0, 4, 12, -2 ** 31], [0, 1]), ([2 ** 31 - 1, 4, 9, 12], [1, 2])]
+
+
+@pytest.mark.parametrize("cu,good", BAD_OFFSETS)
+@pytest.mark.parametrize("causal,S", [(False, 300), (True, 0), (False, 5000)])
+def test_attention_questions_with_bad_offsets(G, cu, good, causal, S):
+    """A sequence whose offsets fall or leave the batch is left out and reported; the sound ones beside it are computed, and rows that
+    belong to none stay as they were. ([0, 5, 3, 12]: rows 3 and 4 would be two sequences' and are not looked at.)"""
+    import torch
+    c = Questions([5, 4, 3], S, 16, 2, 128, causal, False, behind=0)
+    c.cu.copy_(torch.tensor(cu, dtype=torch.int32))
+    c.launch(G)
+    torch.cuda.synchronize()
+    assert int(c.err.item()) == 8
+    ks, vs = values(*c.cache[:2])[:S], values(*c.cache[2:])[:S]
+    taken = set()
+    for i, (a, b) in enumerate(zip(cu, cu[1:])):
+        if not 0 <= a <= b <= c.T:
+            continue
+        taken |= set(range(a, b))
+        if i not in good:
+            continue
+        stop = 3 if cu[:3] == [0, 5, 3] else b  # its later rows are another sequence's too
+        n = b - a
+        k, v = (torch.cat((x, y[a:b].double().reshape(n, 2, 128))) for x, y in ((ks, c.k), (vs, c.v)))
+        seen = torch.ones(n, S + n, dtype=torch.bool, device="cuda")
+        if causal:
+            seen[:, S:] = seen[:, S:].tril()
+        want, spread = attend(c.q[a:b], k, v, seen)
+        close(c.out[a:stop], want[:stop - a], spread[:stop - a])
+    rest = [t for t in range(c.T) if t not in taken]
+    assert (c.out[rest] == -7.0).all()
+
+
+@pytest.mark.parametrize("causal,S", [(False, 300), (True, 0), (False, 5000)])
+def test_attention_questions_with_offsets_that_cover_the_batch_many_times(G, causal, S):
+    """Falling offsets whose sound pairs hold far more tokens than the batch: reported, nothing computed, nothing written."""
+    import torch
+    c = Questions([1] * 400, S, 16, 2, 128, causal, False, behind=0)
+    c.cu.copy_(torch.tensor([400 * (i % 2) for i in range(401)], dtype=torch.int32))
+    c.launch(G)
+    torch.cuda.synchronize()
+    assert int(c.err.item()) == 8
+    assert (c.out == -7.0).all()
+
+
+@pytest.mark.parametrize("cu,good", BAD_OFFSETS)
+def test_attention_decode_with_bad_offsets(G, cu, good):
+    import torch
+    c = Decode([50, 3000, 70], [5, 4, 3], 16, 2, 128, behind=0)
+    c.cu.copy_(torch.tensor(cu, dtype=torch.int32))
+    c.launch(G)
+    torch.cuda.synchronize()
+    assert int(c.err.item()) == 8
+    k, v = values(*c.cache[:2]), values(*c.cache[2:])
+    taken = set()
+    for i, (a, b) in enumerate(zip(cu, cu[1:])):
+        if not 0 <= a <= b <= c.T:
+            continue
+        taken |= set(range(a, b))
+        if i not in good or cu[:3] == [0, 5, 3]:
+            continue
+        s, n, L = c.start[i], c.lens[i], b - a
+        seen = torch.arange(n, device="cuda")[None] <= (n - L + torch.arange(L, device="cuda"))[:, None]
+        close(c.out[a:b], *attend(c.q[a:b].reshape(L, 16, 128), k[s:s + n], v[s:s + n], seen))
+    rest = [t for t in range(c.T) if t not in taken]
+    assert (c.out[rest] == -7.0).all()
+
+
+def test_attention_decode_many_sequences(G):
+    """More sequences than a CTA has threads, most of them short, under a bound far above them."""
+    c = Decode([(13 * i) % 71 for i in range(600)], 1, 4, 1, 64, max_len=1 << 14)
+    c.launch(G)
+    c.check()
+
+
 def test_attention_same_bits_every_run(G):
     import torch
     for c in (Questions([40, 90, 1], 3000, 24, 4, 256, False, True), Questions([200, 31], 0, 16, 2, 128, True, False), Decode([5000, 77, 1234], 2, 24, 4, 256)):

@@ -65,6 +65,7 @@ def test_attention_refusals(dcd):
     for base, name in ((QUESTIONS, "dcd_k_attention_kv4"), (DECODE, "dcd_k_attention_kv4_decode")):
         assert refused(dcd, name, list({**base, "gate": BUF, "gs": 2047}.values()))
         assert refused(dcd, name, list({**base, "gate": ODD, "gs": 2048}.values()))
+        assert refused(dcd, name, list({**base, "gate": BUF, "gs": (1 << 24) + 8}.values()))
     lib = _lib.load()
     for base, name, n in ((QUESTIONS, "dcd_k_attention_kv4", "S"), (DECODE, "dcd_k_attention_kv4_decode", "max_len")):
         size = getattr(lib, name + "_workspace")
