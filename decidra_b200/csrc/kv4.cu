@@ -148,6 +148,7 @@ __device__ __forceinline__ void decode16(const uint2 w, uint8_t scale, T* dst) {
 template <typename T, typename I>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Cache c, size_t cache_rows, const int64_t* __restrict__ slots, T* __restrict__ k,
                                                        T* __restrict__ v, I total, uint32_t groups, int* err) {
+  dependents_start();
   const I i = (I)blockIdx.x * 256 + threadIdx.x;
   if (i >= total) return;
   size_t at = i;

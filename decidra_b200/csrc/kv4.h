@@ -13,6 +13,28 @@ struct Kv4Cache {
   Kv4Part k, v;
 };
 
+// A kernel that may start while the one in front of it in the stream still runs: it does what needs nothing of that one, then waits for
+// it (dependency_wait, in at least one thread of every block) and reads its results. The one in front lets it start with
+// dependents_start; launched the ordinary way, either instruction does nothing.
+#ifdef __CUDACC__
+__device__ __forceinline__ void dependents_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s, const A&... args) {
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c{};
+  c.gridDim = grid;
+  c.blockDim = threads;
+  c.dynamicSmemBytes = smem;
+  c.stream = s;
+  c.attrs = &at;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, args...);
+}
+#endif
+
 inline bool kv4_head_dim_ok(int hd) { return hd == 64 || hd == 128 || hd == 256; }
 
 // slots[i]: the cache row of token i (negative: the token is left out); null: row i.

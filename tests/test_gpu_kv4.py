@@ -634,6 +634,25 @@ def test_attention_in_graphs_and_on_streams(G):
         b.check()
 
 
+def test_attention_questions_captured_and_replayed(G):
+    """The state's decoding and the attention that starts under it, in one graph: replayed with another state and other offsets."""
+    import torch
+    for c in (Questions([33, 20, 0], 700, 24, 4, 256, False, True), Questions([5, 2, 1], 5000, 16, 2, 128, True, False)):
+        c.launch(G)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            c.launch(G, C.c_void_p(torch.cuda.current_stream().cuda_stream))
+        for seed, lens in ((1, c.lens), (2, [c.lens[0] - 3, 3, c.lens[1] + c.lens[2]])):
+            for old, new in zip(c.cache, random_cache(gen(seed), c.S + 2, c.kv, c.hd)):
+                old[:c.S] = new[:c.S]
+            c.lens = lens
+            c.cu.copy_(torch.tensor(cu_of(lens), dtype=torch.int32))
+            c.out.fill_(-7.0)
+            graph.replay()
+            c.check()
+
+
 def test_layer_step_with_all_of_them(G):
     """One low-precision attention layer as a server runs it: residual + norm to e4m3, the FP8 product to q/k/v, the state's K/V into
     the cache, questions over it; then new tokens appended and attended to. Every step against 64 bits on what the step was given."""
