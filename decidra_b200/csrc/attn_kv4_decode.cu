@@ -145,21 +145,30 @@ __device__ __forceinline__ int rounds_of(const Sequence& s, int G) { return (s.L
 // Blocks of one pair of the sequence: at least one, so that the tokens of an empty stretch get their zeros.
 __device__ __forceinline__ int blocks_of(const Sequence& s) { return max(1, (s.len + KB - 1) / KB); }
 
-// PER consecutive values of a row from dimension d: normalised, gated, rounded once
+// PER consecutive values of a row from dimension d: normalised, gated, rounded once; stored N at a time
 template <int PER>
 __device__ __forceinline__ void store_row(const Kv4DecodeArgs& a, const float (&acc)[PER], float sum, size_t at, int t, int h, int hd, int d) {
   const float inv = sum > 0.f ? 1.0f / sum : 0.f;
   const bf16* gate = a.gate_qg ? a.gate_qg + (size_t)t * a.qg_stride + (size_t)(2 * h + 1) * hd + d : nullptr;
   bf16* out = a.out + at * hd + d;
+  constexpr int N = PER < 8 ? PER : 8;
+  struct alignas(2 * N) Values {
+    __nv_bfloat162 two[N / 2];
+  };
 #pragma unroll
-  for (int i = 0; i < PER; i += 2) {
-    float x = acc[i] * inv, y = acc[i + 1] * inv;
-    if (gate) {
-      const __nv_bfloat162 gv = *reinterpret_cast<const __nv_bfloat162*>(gate + i);
-      x *= sigmoid_f(__low2float(gv));
-      y *= sigmoid_f(__high2float(gv));
+  for (int i = 0; i < PER; i += N) {
+    Values gv, v;
+    if (gate) gv = *reinterpret_cast<const Values*>(gate + i);
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      float x = acc[i + j] * inv, y = acc[i + j + 1] * inv;
+      if (gate) {
+        x *= sigmoid_f(__low2float(gv.two[j / 2]));
+        y *= sigmoid_f(__high2float(gv.two[j / 2]));
+      }
+      v.two[j / 2] = __floats2bfloat162_rn(x, y);
     }
-    *reinterpret_cast<__nv_bfloat162*>(out + i) = __floats2bfloat162_rn(x, y);
+    *reinterpret_cast<Values*>(out + i) = v;
   }
 }
 
@@ -281,7 +290,19 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<HD, NT>::CTAS) kv4_decode_kern
       }
     };
 
-    // ---- the first block is on its way before Q is read -----------------------------------------
+    // ---- Q is asked for in front of the first block: behind all CTAs' first blocks it would come last -----------------------------
+    uint4 qw[NT][KW];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = r0 + nt * 8 + g;
+      const bool live = row < n_rows;
+      const bf16* src = live ? a.q + (size_t)(sq.off + row / G) * a.q_stride + (size_t)(kh * G + row % G) * HD : a.q;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        const int d = HD == 256 ? (w >> 2) * 128 + 32 * c + 8 * (w & 3) : KL * 8 * c + 8 * w;
+        qw[nt][w] = live ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
+      }
+    }
     if (first < n_blocks) fetch(first, false);
     cp_commit();
     if (first < n_blocks) fetch(first, true);
@@ -292,16 +313,10 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<HD, NT>::CTAS) kv4_decode_kern
     int end[NT][2];  // first key (relative to the chunk) that the row does not see
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = r0 + nt * 8 + g;
-      const bool live = row < n_rows;
-      const bf16* src = live ? a.q + (size_t)(sq.off + row / G) * a.q_stride + (size_t)(kh * G + row % G) * HD : a.q;
-      uint4 u[KW];
       float m = 0.f;
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
-        const int d = HD == 256 ? (w >> 2) * 128 + 32 * c + 8 * (w & 3) : KL * 8 * c + 8 * w;
-        u[w] = live ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u[w]);
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&qw[nt][w]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(fabsf(__low2float(h[i])), fabsf(__high2float(h[i]))));
       }
@@ -312,7 +327,7 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<HD, NT>::CTAS) kv4_decode_kern
       const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u[w]);
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&qw[nt][w]);
         uint32_t v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = pack_f16(__low2float(h[i]) * inv, __high2float(h[i]) * inv);
@@ -516,6 +531,46 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<HD, NT>::CTAS) kv4_decode_kern
       cp_commit();
     }
     cp_wait<0>();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], 4);
+        l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], 8);
+        l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], 16);
+      }
+    // ---- a warp that has its head to itself writes its rows from registers and goes on: lane (g, c) holds the HD / 8 dimensions from
+    // g * (HD / 8) on, two per t, of rows 2c, 2c + 1 (one token over 2048 rows: 15.3 -> 14.4 us, 64 sequences 149 -> 147; with more column
+    // tiles the registers are short, and four drafted tokens took 34.7 instead of 32.6) -----------------------------------------------
+    if (NT == 1 && hc == WARPS) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = r0 + nt * 8 + 2 * c + i;
+          if (r >= n_rows) continue;
+          const int tt = r / G, tok = sq.off + tt, h = kh * G + r - tt * G;
+          const size_t at = (size_t)tok * a.heads + h;
+          if (part == 0 && g == 0) p.ws_n[at] = n_parts;
+          if (n_parts > 1) {
+            if (g == 0) p.ws_ml[at * p.max_parts + part] = make_float2(m[nt][i], l[nt][i]);
+            float* dst = p.ws_o + (at * p.max_parts + part) * HD + g * (HD / 8);
+#pragma unroll
+            for (int t = 0; t < HD / 16; t += 2)
+              *reinterpret_cast<float4*>(dst + 2 * t) = make_float4(o[t][nt][i], o[t][nt][i + 2], o[t + 1][nt][i], o[t + 1][nt][i + 2]);
+          } else {
+            float acc[HD / 8];
+#pragma unroll
+            for (int t = 0; t < HD / 16; ++t) {
+              acc[2 * t] = o[t][nt][i];
+              acc[2 * t + 1] = o[t][nt][i + 2];
+            }
+            store_row<HD / 8>(a, acc, l[nt][i], at, tok, h, HD, g * (HD / 8));
+          }
+        }
+      __syncwarp();
+      continue;
+    }
     __syncthreads();  // the blocks are done with: the warps' parts take their place
 
     // ---- the four warps' parts of each row. Dimension g * (HD / 8) + 2 t + e lies at t * 16 + 2 g + e, and rows are HD + 4 floats
@@ -528,9 +583,6 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<HD, NT>::CTAS) kv4_decode_kern
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], 4);
-        l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], 8);
-        l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], 16);
         const int row = nt * 8 + 2 * c + i;
         if (g == 0) part_ml[warp * ROWS + row] = make_float2(m[nt][i], l[nt][i]);
         float* dst = part_o + (warp * ROWS + row) * PITCH + 2 * g;
@@ -599,7 +651,7 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<HD, NT>::CTAS) kv4_decode_kern
         }
       }
     };
-    if (hc == 4) rows_out(std::integral_constant<int, 1>(), std::integral_constant<int, HD == 256 ? 3 : 4>());
+    if (NT > 1 && hc == 4) rows_out(std::integral_constant<int, 1>(), std::integral_constant<int, HD == 256 ? 3 : 4>());
     else if (hc == 2) rows_out(std::integral_constant<int, 2>(), std::integral_constant<int, HD == 256 ? 3 : 4>());
     else rows_out(std::integral_constant<int, 4>(), std::integral_constant<int, 2>());
     if (u < u_end) __syncthreads();  // before the next pair's blocks come
