@@ -77,6 +77,21 @@ __device__ __forceinline__ float gate_of(float g) {
   return r;
 }
 
+// Two f32 operations an instruction, each rounded as by itself: the softmax and the issuing warp share the issue slots (64 questions 336 -> 327 us,
+// a tile at head_dim 128 877 -> 820 ns)
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 struct Params {
   const int32_t* cu;
   int B, T, n_state, heads, kv;
@@ -612,7 +627,8 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         m = now;
       }
       const float neg = now == -INFINITY ? 0.f : -now;  // a row that has seen nothing: every weight 2^-inf
-      float l4[4] = {0.f, 0.f, 0.f, 0.f};
+      const float2 scale2 = make_float2(p.scale_log2e, p.scale_log2e), neg2 = make_float2(neg, neg);
+      float2 l2[2] = {};
 #pragma unroll 1
       for (int c = 0; c < KT; c += 64) {
         uint32_t w[32];
@@ -632,14 +648,14 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         }
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          const float a = ex2(fmaf(x[2 * i], p.scale_log2e, neg)), b = ex2(fmaf(x[2 * i + 1], p.scale_log2e, neg));
-          l4[(2 * i) & 3] += a;
-          l4[(2 * i + 1) & 3] += b;
-          w[i] = pack_bf16(a, b);
+          float2 e = fma2(make_float2(x[2 * i], x[2 * i + 1]), scale2, neg2);
+          e = make_float2(ex2(e.x), ex2(e.y));
+          l2[i & 1] = add2(l2[i & 1], e);
+          w[i] = pack_bf16(e.x, e.y);
         }
         tmem_st32(s_tmem + c / 2, w);
       }
-      l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+      l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(bar_p + 8 * b);
