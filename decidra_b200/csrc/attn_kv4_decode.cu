@@ -8,7 +8,7 @@
 // cost 17 % more DRAM traffic than they hold. Each warp has room for one block of its own in shared memory (cp.async, no barrier between
 // warps): the next K is on its way from the end of the S products on, the next V from the end of the P.V products, so that half a block
 // per warp is always in flight and twelve warps fit on an SM (two and three whole blocks a warp and eight warps: 162 us where this takes
-// 149, half of the issue slots empty). Few query rows share each key (tokens x heads of the group, eight per MMA column tile), so the
+// 147, half of the issue slots empty). Few query rows share each key (tokens x heads of the group, eight per MMA column tile), so the
 // kernel lives on getting 0.5625 bytes a value from HBM into matrix fragments:
 //   S^T[16 keys, 8 rows]  += K[16 keys, 16 dims] Q^T      mma.m16n8k16 with the KEYS as the 16-row operand: all of it is used
 //   O^T[16 dims, 8 rows]  += V^T[16 dims, 16 keys] P^T    even for one token of six heads, where rows as M would fill 6 of 16
@@ -22,6 +22,11 @@
 // Q is bf16 and the products f16: each row is divided by the power of two of its largest value (exact but for elements below 2^-14 of
 // it, which keep an absolute error of 2^-25 of it), and the factor returns in the softmax scale. P is held as p * 2^10 in f16, so
 // that weights down to 2^-34 of the row's largest survive. Maxima, sums and O are f32.
+//
+// What bounds it: 64 sequences of 1024 to 16384 rows of 4 heads of 256 take 147 us, 4.3 TB/s (97 us at the copy rate). Of 1190 instructions
+// per 32 keys and head 512 convert and scale codes; 0.57 are issued a cycle and scheduler, the ALU pipe is 54 % busy, and 5 % of the stalls
+// wait for memory: the registers hold three warps a scheduler, and no more of them would fit. One token over 2048 rows takes 14.5 us, all
+// latency.
 //
 // A pair that lies in one CTA is finished there; the parts of one that is cut leave their unnormalised O with maximum and sum in the
 // workspace, and a second kernel adds them up in their order. Keys beyond the stretch are zero-filled, masked keys get p = 0.
