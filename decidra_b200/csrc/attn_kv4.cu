@@ -170,9 +170,13 @@ struct Keys {
   __device__ __forceinline__ Keys(const Params& p, const Tile& t, int part, int parts) {
     n_st = (p.n_state + KT - 1) / KT;
     const int all = n_st + ((p.causal ? t.t0 + t.ntok : t.L) + KT - 1) / KT;
-    const int per = (all + parts - 1) / parts;
-    lo = part * per;
-    n = max(0, min(all, lo + per) - lo);
+    lo = 0;
+    n = all;
+    if (parts > 1) {  // a division of its own latency between two items
+      const int per = (all + parts - 1) / parts;
+      lo = part * per;
+      n = max(0, min(all, lo + per) - lo);
+    }
   }
   __device__ __forceinline__ bool state(int j) const { return lo + j < n_st; }
   __device__ __forceinline__ int key0(int j) const { return (state(j) ? lo + j : lo + j - n_st) * KT; }
@@ -220,15 +224,18 @@ struct Item {
   __device__ __forceinline__ Item(const Params& p, const int2* table, int k, int total) {
     const int nh = p.kv * p.sub, w = item_of(p, k), rest = w / nh;
     hg = w - rest * nh;
-    z = rest / total;
-    ti = tile_of(p, rest - z * total, total);
+    z = ti = 0;  // only parts have a use for them
+    if (p.parts > 1) {
+      z = rest / total;
+      ti = tile_of(p, rest - z * total, total);
+    }
     // uniform for the compiler too, so that what the issuing warps compute from it stays on the uniform datapath
     const int b = __shfl_sync(0xffffffffu, table[k].x, 0);
     tile.t0 = __shfl_sync(0xffffffffu, table[k].y, 0);
     tile.off = p.cu[b];
     tile.L = p.cu[b + 1] - tile.off;
     tile.ntok = min(p.tokens, tile.L - tile.t0);
-    kh = hg / p.sub;
+    kh = p.sub == 1 ? hg : hg / p.sub;
     head0 = kh * (p.heads / p.kv) + (hg - kh * p.sub) * p.G;
   }
 };
