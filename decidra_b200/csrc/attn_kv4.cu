@@ -31,7 +31,7 @@
 //
 // Few items over many keys leave SMs idle; the key tiles are then split into parts, items of their own, which a second kernel adds up.
 //
-// 64 questions of about 107 tokens over 2048 rows, 24 heads of 256, gated: 327 us, 1080 TFLOP/s of the 1648 that a library product reaches;
+// 64 questions of about 107 tokens over 2048 rows, 24 heads of 256, gated: 322 to 333 us, 1080 TFLOP/s of the 1648 that a library product reaches;
 // the tensor pipe is busy 56 % of the time, a tile takes 2400 to 2600 cycles for 2048 of products (S[j + 2] waits for P.V[j]), and a
 // quarter of an item is its start, its masked tile and its rows. Five causal prompts of 1051 to 1814 tokens, 16 heads of 128: 67 to 83 us,
 // bounded by the issue slots that the softmax and the issuing warp share.
