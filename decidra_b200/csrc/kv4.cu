@@ -119,8 +119,8 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(const T* __restrict__ k,
   v_scales[at] = scale;
 }
 
-// e2m1 * e4m3 is exact in f16, and in either output type
-template <typename T>
+// e2m1 * e4m3 is exact in f16, and in either output type. ALIGN: 32-byte stores, or 16-byte ones
+template <typename T, int ALIGN>
 __device__ __forceinline__ void decode16(const uint2 w, uint8_t scale, T* dst) {
   const __half_raw hr = __nv_cvt_fp8_to_halfraw(scale, __NV_E4M3);
   const __half2 s2 = __half2half2(*reinterpret_cast<const __half*>(&hr));
@@ -142,11 +142,17 @@ __device__ __forceinline__ void decode16(const uint2 w, uint8_t scale, T* dst) {
     uint32_t q[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) q[i] = u[8 * h + i];
-    st256(reinterpret_cast<uint32_t*>(dst) + 8 * h, q);
+    if constexpr (ALIGN == 32) {
+      st256(reinterpret_cast<uint32_t*>(dst) + 8 * h, q);
+    } else {
+      uint4* d = reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(dst) + 8 * h);
+      d[0] = make_uint4(q[0], q[1], q[2], q[3]);
+      d[1] = make_uint4(q[4], q[5], q[6], q[7]);
+    }
   }
 }
 
-template <typename T, typename I>
+template <typename T, int ALIGN, typename I>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Cache c, size_t cache_rows, const int64_t* __restrict__ slots, T* __restrict__ k,
                                                        T* __restrict__ v, I total, uint32_t groups, int* err) {
   dependents_start();
@@ -161,8 +167,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Cache c, size_t 
   }
   const uint2 wk = reinterpret_cast<const uint2*>(c.k.codes)[at], wv = reinterpret_cast<const uint2*>(c.v.codes)[at];
   const uint8_t sk = c.k.scales[at], sv = c.v.scales[at];
-  decode16<T>(wk, sk, k + (size_t)i * 16);
-  decode16<T>(wv, sv, v + (size_t)i * 16);
+  decode16<T, ALIGN>(wk, sk, k + (size_t)i * 16);
+  decode16<T, ALIGN>(wv, sv, v + (size_t)i * 16);
 }
 
 }  // namespace
@@ -194,8 +200,10 @@ cudaError_t launch_kv4_read(const Kv4Cache& c, size_t cache_rows, const int64_t*
   const uint32_t groups = (uint32_t)kv * (hd / 16);
   const size_t total = (size_t)rows * groups;
   const unsigned grid = (unsigned)((total + 255) / 256);
-  if (total >= (1u << 31)) kv4_read_kernel<T, size_t><<<grid, 256, 0, s>>>(c, cache_rows, slots, k, v, total, groups, err);
-  else kv4_read_kernel<T, uint32_t><<<grid, 256, 0, s>>>(c, cache_rows, slots, k, v, (uint32_t)total, groups, err);
+  const bool wide = (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 32 == 0;
+  if (total >= (1u << 31)) kv4_read_kernel<T, 16, size_t><<<grid, 256, 0, s>>>(c, cache_rows, slots, k, v, total, groups, err);
+  else if (wide) kv4_read_kernel<T, 32, uint32_t><<<grid, 256, 0, s>>>(c, cache_rows, slots, k, v, (uint32_t)total, groups, err);
+  else kv4_read_kernel<T, 16, uint32_t><<<grid, 256, 0, s>>>(c, cache_rows, slots, k, v, (uint32_t)total, groups, err);
   return cudaGetLastError();
 }
 #define INST_KV4(T)                                                                                                                                     \

@@ -273,7 +273,7 @@ cudaError_t launch(const T* x, size_t xs, const T* mix, size_t ms, const T* w, T
       rmsnorm_fp8_long_kernel<T, ADD, true><<<rows, 256, 0, s>>>(x, xs, mix, ms, w, res, out, scales, cols, eps, wofs, clip);
   } else {
     auto threads = [](int items, int per) { return ((items + per - 1) / per + 31) / 32 * 32; };
-    if (wide && cols <= V * 1024) {
+    if (wide && cols <= V * 1024 && rows <= 1 << 30) {  // the row number may pass `rows` by the grid
       const int nt = threads(cols / V, 1);
       const int grid = min(rows, sm_count() * (ROWS_THREADS / nt));
       rmsnorm_fp8_rows_kernel<T, V, ADD><<<grid, nt, 0, s>>>(x, xs, mix, ms, w, res, out, scales, rows, cols, eps, wofs, clip);

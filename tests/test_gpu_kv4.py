@@ -192,6 +192,46 @@ def test_cache_rows_in_order_and_the_bits_of_the_nvfp4_rows(G):
         assert torch.equal(out, two[0]) and torch.equal(out, two[1])
 
 
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_cache_read_to_rows_of_16_byte_alignment(G, dtype):
+    """What the interface asks for is 16 bytes: outputs, and an attention's workspace, that are not on 32."""
+    import torch
+    rows, kv, hd = 37, 2, 128
+    cache = random_cache(gen(9), rows, kv, hd)
+    t, skip = (torch.bfloat16, 8) if dtype else (torch.float32, 4)
+    k, v = (torch.full((rows * kv * hd + 2 * skip,), -7.0, dtype=t, device="cuda") for _ in range(2))
+    for shift_k, shift_v in ((skip, skip), (0, skip), (skip, 0)):
+        a, b = k[shift_k:shift_k + rows * kv * hd], v[shift_v:shift_v + rows * kv * hd]
+        G.call("dcd_k_kv4_read", *cache, rows, None, a, b, rows, kv, hd, dtype, None, None)
+        torch.cuda.synchronize()
+        assert torch.equal(a.double().reshape(rows, kv, hd), values(*cache[:2])) and torch.equal(b.double().reshape(rows, kv, hd), values(*cache[2:]))
+    assert (k[-skip:] == -7.0).all() and (v[-skip:] == -7.0).all()
+
+
+@pytest.mark.parametrize("form", ["questions", "prompts", "decode"])
+def test_attention_operands_of_16_byte_alignment(G, form):
+    import torch
+    c = {"questions": lambda: Questions([40, 3], 5000, 16, 2, 128, False, True), "prompts": lambda: Questions([40, 300], 0, 24, 4, 256, True, True),
+         "decode": lambda: Decode([5000, 40], 1, 24, 4, 256)}[form]()
+
+    def shifted(x):  # the same values 16 bytes further on
+        if x is None or not isinstance(x, torch.Tensor):
+            return x
+        skip = 16 // x.element_size()
+        whole = torch.empty(x.untyped_storage().nbytes() // x.element_size() + skip, dtype=x.dtype, device="cuda")
+        return torch.as_strided(whole, x.shape, x.stride(), skip + x.storage_offset()).copy_(x)
+
+    c.launch(G)  # makes the workspace
+    c.q, c.gate, c.out, c.cache = shifted(c.q), shifted(c.gate), shifted(c.out), [shifted(x) for x in c.cache]
+    if form != "decode":
+        c.k, c.v = shifted(c.k), shifted(c.v)
+    c.ws = torch.full((c.ws.numel() + 16,), 0xFF, dtype=torch.uint8, device="cuda")[16:]
+    c.out.fill_(-7.0)
+    assert all(x.data_ptr() % 32 == 16 for x in (c.q, c.out, c.ws, *c.cache))
+    c.launch(G)
+    c.check()
+
+
 def test_cache_values_that_are_not_finite_stay_in_their_group(G):
     import torch
     rows, kv, hd = 3, 1, 64
