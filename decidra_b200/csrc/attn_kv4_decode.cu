@@ -8,7 +8,7 @@
 // cost 17 % more DRAM traffic than they hold. Each warp has room for one block of its own in shared memory (cp.async, no barrier between
 // warps): the next K is on its way from the end of the S products on, the next V from the end of the P.V products, so that half a block
 // per warp is always in flight and twelve warps fit on an SM (two and three whole blocks a warp and eight warps: 162 us where this takes
-// 147, half of the issue slots empty). Few query rows share each key (tokens x heads of the group, eight per MMA column tile), so the
+// 144, half of the issue slots empty). Few query rows share each key (tokens x heads of the group, eight per MMA column tile), so the
 // kernel lives on getting 0.5625 bytes a value from HBM into matrix fragments:
 //   S^T[16 keys, 8 rows]  += K[16 keys, 16 dims] Q^T      mma.m16n8k16 with the KEYS as the 16-row operand: all of it is used
 //   O^T[16 dims, 8 rows]  += V^T[16 dims, 16 keys] P^T    even for one token of six heads, where rows as M would fill 6 of 16
@@ -23,15 +23,13 @@
 // it, which keep an absolute error of 2^-25 of it), and the factor returns in the softmax scale. P is held as p * 2^10 in f16, so
 // that weights down to 2^-34 of the row's largest survive. Maxima, sums and O are f32.
 //
-// What bounds it: 64 sequences of 1024 to 16384 rows of 4 heads of 256 take 147 us, 4.3 TB/s (97 us at the copy rate). Of 1190 instructions
+// What bounds it: 64 sequences of 1024 to 16384 rows of 4 heads of 256 take 144 us, 4.4 TB/s (97 us at the copy rate). Of 1190 instructions
 // per 32 keys and head 512 convert and scale codes; 0.57 are issued a cycle and scheduler, the ALU pipe is 54 % busy, and 5 % of the stalls
-// wait for memory: the registers hold three warps a scheduler, and no more of them would fit. One token over 2048 rows takes 14.5 us, all
+// wait for memory: the registers hold three warps a scheduler, and no more of them would fit. One token over 2048 rows takes 14.3 us, all
 // latency.
 //
-// A pair that lies in one CTA is finished there; the parts of one that is cut leave their unnormalised O with maximum and sum in the
+// Rows whose keys all went through one warp are finished there; otherwise each warp leaves its unnormalised O with maximum and sum in the
 // workspace, and a second kernel adds them up in their order. Keys beyond the stretch are zero-filled, masked keys get p = 0.
-#include <type_traits>
-
 #include "common.cuh"
 #include "kv4.h"
 
@@ -111,7 +109,7 @@ struct Args {
   Kv4DecodeArgs a;
   int hc;          // K/V heads of a pair: 4, 2 or 1
   int q_min;       // least blocks per CTA
-  int max_parts;   // parts of a pair, at most: max_len in blocks / q_min, and one more for its offset
+  int max_parts;   // parts of a row, at most: max_len in blocks / q_min, and one more for its offset, times the warps of a head
   float* ws_o;     // [T * heads][max_parts][hd]
   float2* ws_ml;   // [T * heads][max_parts] (maximum in log2 units, sum)
   int* ws_n;       // [T * heads] parts of the row's pair
@@ -544,122 +542,36 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<HD, NT>::CTAS) kv4_decode_kern
         l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], 8);
         l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], 16);
       }
-    // ---- a warp that has its head to itself writes its rows from registers and goes on: lane (g, c) holds the HD / 8 dimensions from
-    // g * (HD / 8) on, two per t, of rows 2c, 2c + 1 (one token over 2048 rows: 15.3 -> 14.4 us, 64 sequences 149 -> 147; with more column
-    // tiles the registers are short, and four drafted tokens took 34.7 instead of 32.6) -----------------------------------------------
-    if (NT == 1 && hc == WARPS) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = r0 + nt * 8 + 2 * c + i;
-          if (r >= n_rows) continue;
-          const int tt = r / G, tok = sq.off + tt, h = kh * G + r - tt * G;
-          const size_t at = (size_t)tok * a.heads + h;
-          if (part == 0 && g == 0) p.ws_n[at] = n_parts;
-          if (n_parts > 1) {
-            if (g == 0) p.ws_ml[at * p.max_parts + part] = make_float2(m[nt][i], l[nt][i]);
-            float* dst = p.ws_o + (at * p.max_parts + part) * HD + g * (HD / 8);
-#pragma unroll
-            for (int t = 0; t < HD / 16; t += 2)
-              *reinterpret_cast<float4*>(dst + 2 * t) = make_float4(o[t][nt][i], o[t][nt][i + 2], o[t + 1][nt][i], o[t + 1][nt][i + 2]);
-          } else {
-            float acc[HD / 8];
-#pragma unroll
-            for (int t = 0; t < HD / 16; ++t) {
-              acc[2 * t] = o[t][nt][i];
-              acc[2 * t + 1] = o[t][nt][i + 2];
-            }
-            store_row<HD / 8>(a, acc, l[nt][i], at, tok, h, HD, g * (HD / 8));
-          }
-        }
-      __syncwarp();
-      continue;
-    }
-    __syncthreads();  // the blocks are done with: the warps' parts take their place
-
-    // ---- the four warps' parts of each row. Dimension g * (HD / 8) + 2 t + e lies at t * 16 + 2 g + e, and rows are HD + 4 floats
-    // apart: the sixteen lanes of a store (four g, four rows two apart) then meet sixteen different pairs of banks ----------------
-    constexpr int PITCH = HD + 4;
-    float* part_o = reinterpret_cast<float*>(smem);                                // [warp][row][PITCH]
-    float2* part_ml = reinterpret_cast<float2*>(smem + WARPS * ROWS * PITCH * 4);  // [warp][row]
-    float2* total_ml = part_ml + WARPS * ROWS;                                     // [row][head]
+    // ---- every warp is a part of its rows and writes it from registers: lane (g, c) holds the HD / 8 dimensions from g * (HD / 8) on,
+    // two per t, of rows 2c, 2c + 1. (With a head's warps added up through shared memory first, 64 sequences took 147 us instead of 144,
+    // and nine of four drafted tokens over two heads the same 33: the second kernel has fewer parts then, this one three barriers.)
+    const int parts_all = n_parts * step, my_part = part * step + first;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int row = nt * 8 + 2 * c + i;
-        if (g == 0) part_ml[warp * ROWS + row] = make_float2(m[nt][i], l[nt][i]);
-        float* dst = part_o + (warp * ROWS + row) * PITCH + 2 * g;
+        const int r = r0 + nt * 8 + 2 * c + i;
+        if (r >= n_rows) continue;
+        const int tt = r / G, tok = sq.off + tt, h = kh * G + r - tt * G;
+        const size_t at = (size_t)tok * a.heads + h;
+        if (my_part == 0 && g == 0) p.ws_n[at] = parts_all;
+        if (parts_all > 1) {
+          if (g == 0) p.ws_ml[at * p.max_parts + my_part] = make_float2(m[nt][i], l[nt][i]);
+          float* dst = p.ws_o + (at * p.max_parts + my_part) * HD + g * (HD / 8);
 #pragma unroll
-        for (int t = 0; t < HD / 16; ++t) *reinterpret_cast<float2*>(dst + 16 * t) = make_float2(o[t][nt][i], o[t][nt][i + 2]);
-      }
-    __syncthreads();
-    // every (head, row): the maximum and sum over the head's warps hs, hs + hc, ..., and the warps' weights in place of their maxima
-    const int rows_here = min(ROWS, n_rows - r0), n_out = rows_here * hc;
-    for (int i = threadIdx.x; i < n_out; i += WARPS * 32) {
-      const int row = i / hc, hs = i - row * hc;
-      float M = -INFINITY, sum = 0.f;
-      for (int w = hs; w < WARPS; w += hc) M = fmaxf(M, part_ml[w * ROWS + row].x);
-      for (int w = hs; w < WARPS; w += hc) {
-        const float2 ml = part_ml[w * ROWS + row];
-        const float fw = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-        sum += fw * ml.y;
-        part_ml[w * ROWS + row].x = fw;
-      }
-      total_ml[i] = make_float2(M, sum);
-    }
-    __syncthreads();
-    constexpr int PER = HD / 32;  // consecutive values of a lane; one warp per row
-    const int d0 = lane * PER, at0 = d0 % (HD / 8) * 8 + d0 / (HD / 8) * 2;
-    // WK warps of a head, IL rows of a warp at a time
-    auto rows_out = [&](auto wk, auto il) {
-      constexpr int WK = decltype(wk)::value, IL = decltype(il)::value;
-      for (int i0 = warp; i0 < n_out; i0 += WARPS * IL) {
-        float acc[IL][PER];
-        int hs[IL], row[IL];
+          for (int t = 0; t < HD / 16; t += 2)
+            *reinterpret_cast<float4*>(dst + 2 * t) = make_float4(o[t][nt][i], o[t][nt][i + 2], o[t + 1][nt][i], o[t + 1][nt][i + 2]);
+        } else {
+          float acc[HD / 8];
 #pragma unroll
-        for (int n = 0; n < IL; ++n) {
-          const int i = min(i0 + n * WARPS, n_out - 1);
-          row[n] = i / (WARPS / WK);
-          hs[n] = i % (WARPS / WK);
-#pragma unroll
-          for (int j = 0; j < PER; ++j) acc[n][j] = 0.f;
-#pragma unroll
-          for (int v = 0; v < WK; ++v) {
-            const int w = hs[n] + v * (WARPS / WK);
-            const float fw = part_ml[w * ROWS + row[n]].x;
-#pragma unroll
-            for (int j = 0; j < PER; j += 2) {
-              const float2 x = *reinterpret_cast<const float2*>(part_o + (w * ROWS + row[n]) * PITCH + at0 + 8 * j);
-              acc[n][j] += fw * x.x;
-              acc[n][j + 1] += fw * x.y;
-            }
+          for (int t = 0; t < HD / 16; ++t) {
+            acc[2 * t] = o[t][nt][i];
+            acc[2 * t + 1] = o[t][nt][i + 2];
           }
-        }
-#pragma unroll
-        for (int n = 0; n < IL; ++n) {
-          const int i = i0 + n * WARPS;
-          if (i >= n_out) break;
-          const float2 ml = total_ml[i];
-          const int r = r0 + row[n], tt = r / G, t = sq.off + tt, h = (kh - my_head + hs[n]) * G + r - tt * G;
-          const size_t at = (size_t)t * a.heads + h;
-          if (part == 0 && lane == 0) p.ws_n[at] = n_parts;
-          if (n_parts > 1) {
-            if (lane == 0) p.ws_ml[at * p.max_parts + part] = ml;
-            float* dst = p.ws_o + (at * p.max_parts + part) * HD + d0;
-#pragma unroll
-            for (int j = 0; j < PER; j += 2) *reinterpret_cast<float2*>(dst + j) = make_float2(acc[n][j], acc[n][j + 1]);
-          } else {
-            store_row<PER>(a, acc[n], ml.y, at, t, h, HD, d0);
-          }
+          store_row<HD / 8>(a, acc, l[nt][i], at, tok, h, HD, g * (HD / 8));
         }
       }
-    };
-    if (NT > 1 && hc == 4) rows_out(std::integral_constant<int, 1>(), std::integral_constant<int, HD == 256 ? 3 : 4>());
-    else if (hc == 2) rows_out(std::integral_constant<int, 2>(), std::integral_constant<int, HD == 256 ? 3 : 4>());
-    else rows_out(std::integral_constant<int, 4>(), std::integral_constant<int, 2>());
-    if (u < u_end) __syncthreads();  // before the next pair's blocks come
+    __syncwarp();  // before the next pair's Q and blocks come
   }
 }
 
@@ -753,15 +665,14 @@ Plan plan_of(int B, int kv, int max_len) {
   const long long blocks = max(1LL, ((long long)max_len + KB - 1) / KB);
   const double share = (double)B * (kv / p.hc) * (double)blocks / (8.0 * p.sms);  // an eighth of what the CTAs of two per SM would take
   p.q_min = (int)max(2LL * WARPS / p.hc, (long long)min(ceil(share), (double)blocks));
-  p.max_parts = (int)((blocks + p.q_min - 1) / p.q_min) + 1;
+  p.max_parts = (int)((blocks + p.q_min - 1) / p.q_min + 1) * (WARPS / p.hc);
   return p;
 }
 
 template <int HD, int NT>
 cudaError_t run(const Args& p, int sms, cudaStream_t s) {
   using C = Cfg<HD, NT>;
-  constexpr int blocks = WARPS * (Block<HD>::BYTES + (C::Q_SMEM ? HD / 16 * NT * 256 : 0)), parts = WARPS * 8 * NT * ((HD + 4) * 4 + 16);
-  constexpr int bytes = blocks > parts ? blocks : parts;
+  constexpr int bytes = WARPS * (Block<HD>::BYTES + (C::Q_SMEM ? HD / 16 * NT * 256 : 0));
   static_assert(C::CTAS * (bytes + 1024 + 256) <= 228 * 1024, "shared memory of an SM");
   CUDA_TRY(cudaFuncSetAttribute(kv4_decode_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   kv4_decode_kernel<HD, NT><<<sms * C::CTAS, WARPS * 32, bytes, s>>>(p);
