@@ -25,7 +25,7 @@
 //
 // What bounds it: 64 sequences of 1024 to 16384 rows of 4 heads of 256 take 144 us, 4.4 TB/s (97 us at the copy rate). Of 1190 instructions
 // per 32 keys and head 512 convert and scale codes; 0.57 are issued a cycle and scheduler, the ALU pipe is 54 % busy, and 5 % of the stalls
-// wait for memory: the registers hold three warps a scheduler, and no more of them would fit. One token over 2048 rows takes 14.3 us, all
+// wait for memory: the registers hold three warps a scheduler, and no more of them would fit. One token over 2048 rows takes 12.7 us, all
 // latency.
 //
 // Rows whose keys all went through one warp are finished there; otherwise each warp leaves its unnormalised O with maximum and sum in the
@@ -576,15 +576,19 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<HD, NT>::CTAS) kv4_decode_kern
 }
 
 // out = sum_z O_z 2^(m_z - M) / sum_z l_z 2^(m_z - M). W warps per (token, head) take the parts in turn; their sums are added in
-// order. The row's sequence is found 32 offsets at a time, and 32 parts' weights come at once, so that little of the kernel is a chain
-// of loads (one after the other they were 28 us for one token over 64 parts).
+// order. The row's sequence is found 32 offsets at a time, 32 parts' weights come at once, and the rows of four or eight parts are asked
+// for before the first is used: a chain of loads is what this kernel's time is made of (both kernels, one token over 8000 rows in 125
+// parts: 17 us; with a loop of one part after the other and never more than four warps 23.5; over 2048 rows 12.7 and 14.3).
 template <int HD, int W>
-__global__ void __launch_bounds__(128) kv4_decode_merge_kernel(const Args p) {
-  constexpr int PER = HD / 32;
-  __shared__ float part[W > 1 ? 4 : 1][HD], part_sum[4];
+__global__ void __launch_bounds__(W > 4 ? W * 32 : 128) kv4_decode_merge_kernel(const Args p) {
+  constexpr int WARPS_HERE = W > 4 ? W : 4, VEC = HD == 64 ? 2 : 4, NV = HD / 32 / VEC, U = W > 4 ? 8 : 4;  // a lane's values: VEC from lane * VEC on, NV times
+  struct alignas(4 * VEC) Values {
+    float f[VEC];
+  };
+  __shared__ float part[W > 1 ? WARPS_HERE : 1][HD], part_sum[WARPS_HERE];
   const Kv4DecodeArgs& a = p.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = warp % W;
-  const size_t at = (size_t)blockIdx.x * (4 / W) + warp / W;
+  const size_t at = (size_t)blockIdx.x * (WARPS_HERE / W) + warp / W;
   const int t = (int)(at / (unsigned)a.heads), h = (int)(at - (size_t)t * a.heads);
   int nz = 0;
   if (t < a.T) {
@@ -599,30 +603,45 @@ __global__ void __launch_bounds__(128) kv4_decode_merge_kernel(const Args p) {
     const int off = a.cu[lo], end = a.cu[lo + 1];
     if (off >= 0 && off <= t && t < end && end <= a.T) nz = p.ws_n[at];
   }
-  if (W == 1 && nz <= 1) return;  // finished by its only CTA, or no token of a sequence
+  if (W == 1 && nz <= 1) return;  // finished by its only warp, or no token of a sequence
   const float2* ml = p.ws_ml + at * p.max_parts;
   float M = -INFINITY;
+#pragma unroll 4
   for (int z = lane; z < nz; z += 32) M = fmaxf(M, ml[z].x);
   M = warp_max(M);
-  float acc[PER], sum = 0.f;
+  float acc[NV][VEC], sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) acc[i][j] = 0.f;
   if (nz > 1 && M != -INFINITY) {
-    const float* src = p.ws_o + at * p.max_parts * HD + lane * PER;
+    const float* src = p.ws_o + at * p.max_parts * HD + lane * VEC;
     for (int z0 = w; z0 < nz; z0 += 32 * W) {  // this warp's next 32 parts: z0, z0 + W, ...
       const int mine = z0 + lane * W;
       const float2 x = mine < nz ? ml[mine] : make_float2(-INFINITY, 0.f);
       const float wt = ex2(x.x - M);  // a part that saw nothing has m = -inf: weight 0 on zeros
       sum += wt * x.y;
       const int n = min(32, (nz - z0 + W - 1) / W);
-#pragma unroll 8
-      for (int z = 0; z < n; ++z) {
-        const float wz = __shfl_sync(0xffffffffu, wt, z);
+      for (int z = 0; z < n; z += U) {
+        Values v[U][NV];
 #pragma unroll
-        for (int i = 0; i < PER; i += 2) {
-          const float2 v = *reinterpret_cast<const float2*>(src + (size_t)(z0 + z * W) * HD + i);
-          acc[i] += wz * v.x;
-          acc[i + 1] += wz * v.y;
+        for (int k = 0; k < U; ++k)
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            if (z + k < n) {
+              v[k][i] = *reinterpret_cast<const Values*>(src + (size_t)(z0 + (z + k) * W) * HD + i * 32 * VEC);
+            } else {
+#pragma unroll
+              for (int j = 0; j < VEC; ++j) v[k][i].f[j] = 0.f;
+            }
+          }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          const float wz = __shfl_sync(0xffffffffu, wt, (z + k) & 31);
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) acc[i][j] += wz * v[k][i].f[j];
         }
       }
     }
@@ -630,21 +649,28 @@ __global__ void __launch_bounds__(128) kv4_decode_merge_kernel(const Args p) {
   }
   if constexpr (W > 1) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) part[warp][lane * PER + i] = acc[i];
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) part[warp][(i * 32 + lane) * VEC + j] = acc[i][j];
     if (lane == 0) part_sum[warp] = sum;
     __syncthreads();
     if (w != 0 || nz <= 1) return;
     sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[i][j] = 0.f;
 #pragma unroll
     for (int v = 0; v < W; ++v) {
       sum += part_sum[warp + v];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) acc[i] += part[warp + v][lane * PER + i];
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[i][j] += part[warp + v][(i * 32 + lane) * VEC + j];
     }
   }
-  store_row<PER>(a, acc, sum, at, t, h, HD, lane * PER);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) store_row<VEC>(a, acc[i], sum, at, t, h, HD, (i * 32 + lane) * VEC);
 }
 
 int sm_count() {
@@ -678,8 +704,10 @@ cudaError_t run(const Args& p, int sms, cudaStream_t s) {
   kv4_decode_kernel<HD, NT><<<sms * C::CTAS, WARPS * 32, bytes, s>>>(p);
   CUDA_TRY(cudaGetLastError());
   const size_t rows = (size_t)p.a.T * p.a.heads;
+  // more warps a row where more parts make a longer chain; fewer where they would have less than a part or two each
   if (p.max_parts <= 8) kv4_decode_merge_kernel<HD, 1><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
-  else kv4_decode_merge_kernel<HD, 4><<<(unsigned)rows, 128, 0, s>>>(p);
+  else if (p.max_parts <= 32) kv4_decode_merge_kernel<HD, 4><<<(unsigned)rows, 128, 0, s>>>(p);
+  else kv4_decode_merge_kernel<HD, 16><<<(unsigned)rows, 512, 0, s>>>(p);
   return cudaGetLastError();
 }
 
