@@ -784,7 +784,7 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 // out = sum_z O_z 2^(m_z - M) / sum_z l_z 2^(m_z - M), gated: one warp per row; grid (tiles, heads' tiles, 128 / 4 rows)
 template <int HD>
 __global__ void __launch_bounds__(128) kv4_attention_merge_kernel(const Params p, int parts) {
-  constexpr int PER = HD / 32;
+  constexpr int PER = HD / 32, U = 8;
   __shared__ int sums[4], found[3];
   if (threadIdx.x == 0) found[0] = -1;
   __syncthreads();
@@ -804,28 +804,44 @@ __global__ void __launch_bounds__(128) kv4_attention_merge_kernel(const Params p
   const int head = kh * (p.heads / p.kv) + (hg - kh * p.sub) * G + r - tt * G;
   const size_t step = (size_t)gridDim.y * gridDim.x * 128, row0 = ((size_t)hg * gridDim.x + blockIdx.x) * 128 + r;
   float M = -INFINITY;
-  for (int z = lane; z < parts; z += 32) {
-    const float2 x = p.ws_ml[z * step + row0];
-    if (x.y > 0.f) M = fmaxf(M, x.x);
+  float2 ml[4];  // parts lane, lane + 32, ... of at most 128
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int z = lane + 32 * k;
+    ml[k] = z < parts ? p.ws_ml[z * step + row0] : make_float2(-INFINITY, 0.f);
+    if (ml[k].y > 0.f) M = fmaxf(M, ml[k].x);
   }
   M = warp_max(M);
   float acc[PER], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-#pragma unroll 4
-  for (int z = 0; z < parts; ++z) {
-    const float2 x = p.ws_ml[z * step + row0];
-    if (!(x.y > 0.f)) continue;  // a part without keys, or one that this row sees nothing of: it may have written no O
-    const float w = ex2(x.x - M);
-    sum += w * x.y;
-    const float* src = p.ws_o + (z * step + row0) * HD + lane * PER;
 #pragma unroll
-    for (int i = 0; i < PER; i += 2) {
-      const float2 v = *reinterpret_cast<const float2*>(src + i);
-      acc[i] += w * v.x;
-      acc[i + 1] += w * v.y;
+  for (int k = 0; k < 4; ++k) {
+    if (32 * k >= parts) break;
+    // a part without keys, or one that this row sees nothing of, may have written no O: weight 0, and its row is not read
+    const float wt = ml[k].y > 0.f ? ex2(ml[k].x - M) : 0.f;
+    sum += wt * ml[k].y;
+    const uint32_t have = __ballot_sync(0xffffffffu, wt > 0.f);
+    const float* src = p.ws_o + (32 * k * step + row0) * HD + lane * PER;
+    for (int z0 = 0; z0 < 32 && 32 * k + z0 < parts; z0 += U) {  // U rows are asked for before the first is used
+      float2 v[U][PER / 2];
+#pragma unroll
+      for (int z = 0; z < U; ++z)
+#pragma unroll
+        for (int i = 0; i < PER / 2; ++i)
+          v[z][i] = have >> (z0 + z) & 1u ? *reinterpret_cast<const float2*>(src + (size_t)(z0 + z) * step * HD + 2 * i) : make_float2(0.f, 0.f);
+#pragma unroll
+      for (int z = 0; z < U; ++z) {
+        const float wz = __shfl_sync(0xffffffffu, wt, z0 + z);
+#pragma unroll
+        for (int i = 0; i < PER / 2; ++i) {
+          acc[2 * i] += wz * v[z][i].x;
+          acc[2 * i + 1] += wz * v[z][i].y;
+        }
+      }
     }
   }
+  sum = warp_sum(sum);
   const size_t t = (size_t)found[0] + found[1] + tt;
   const float inv = sum > 0.f ? 1.0f / sum : 0.f;
   const bf16* gate = p.gate_qg ? p.gate_qg + t * p.qg_stride + (size_t)(2 * head + 1) * HD + lane * PER : nullptr;
