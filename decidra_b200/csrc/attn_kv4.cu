@@ -485,7 +485,8 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         if (i >= SB) {  // O += P[j] V[j]; P[j] lies over S[j]: 16 keys = 8 columns of bf16 pairs
           const int j = i - SB, J = jj + j;
           next_event();  // V[j] and P[j]
-          if (j == 0 && live > 0 && !(ok = mbar_wait_warp(bar_o_free, (uint32_t)(live - 1) & 1, abort_flag))) break;  // O of the item before has been read
+          if (ok && j == 0 && live > 0) ok = mbar_wait_warp(bar_o_free, (uint32_t)(live - 1) & 1, abort_flag);  // O of the item before has been read
+          if (!ok) break;  // the event may have been the last
           const int valid = keys.valid(j, p, it.tile);
           constexpr uint32_t idesc = umma_idesc(128, HD, 1);
           const uint32_t pj = tmem + S_COL + pb * KT;
