@@ -705,6 +705,11 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     float end_m = -INFINITY;
     if (ok) {
       end_m = m_used[last * 128 + r];
+      // The other group may still be reading this group's sums of the item before. With two tiles or more it has published a maximum of this
+      // item since, and that was waited for; the owner of an item's only tile has waited for nothing of the other group.
+      if (n_tiles == 1 && live > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar_o_free, (uint32_t)(live - 1) & 1, abort_flag));
+    }
+    if (ok) {
       l_part[h * 128 + r] = m == -INFINITY ? 0.f : l * ex2(m - end_m);
       mbar_arrive(bar_l);
       ok = __all_sync(0xffffffffu, mbar_wait(bar_l, (uint32_t)live & 1, abort_flag));
