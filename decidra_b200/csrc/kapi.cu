@@ -1,6 +1,9 @@
 // Kernel-level C entry points: raw device pointers in, one launch out. They exist so that every
 // kernel can be checked against the CPU oracle and timed on its own through the C ABI.
 #include "../../include/decidra_b200.h"
+
+#include <initializer_list>
+
 #include "attn_tcgen05.h"
 #include "common.cuh"
 #include "gemm_tcgen05.h"
@@ -10,6 +13,13 @@
 namespace {
 inline int rc_of(cudaError_t e) { return e == cudaSuccess ? DCD_OK : (e == cudaErrorInvalidValue ? DCD_E_INVALID : DCD_E_CUDA); }
 inline cudaStream_t S(void* s) { return reinterpret_cast<cudaStream_t>(s); }
+// pointers on whole elements (a null one is): anything else is a misaligned address on the device
+inline bool whole(size_t element, std::initializer_list<const void*> ptrs) {
+  for (const void* p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) % element != 0) return false;
+  return true;
+}
+inline size_t element_size(int dtype) { return dtype == 0 ? 4 : 2; }
 }  // namespace
 
 #define DISPATCH(dtype, call_f32, call_bf16) ((dtype) == 0 ? rc_of(call_f32) : (dtype) == 1 ? rc_of(call_bf16) : DCD_E_INVALID)
@@ -142,6 +152,7 @@ int dcd_k_add_rmsnorm(const void* x, const void* mix, const void* w, void* resid
 int dcd_k_rmsnorm_fp8(const void* x, size_t x_stride, const void* w, void* out, float* scales, int rows, int cols, float eps, int zero_centered, float clip,
                       int round_t, int dtype, void* stream) {
   if (rows < 0 || cols <= 0 || x_stride < (size_t)cols || !x || !w || !out || !scales) return DCD_E_INVALID;
+  if (!whole(element_size(dtype), {x, w}) || !whole(4, {scales})) return DCD_E_INVALID;
   return DISPATCH(dtype,
                   launch_rmsnorm_fp8<float>((const float*)x, x_stride, nullptr, 0, (const float*)w, nullptr, (uint8_t*)out, scales, rows, cols, eps, zero_centered != 0, clip, round_t != 0, S(stream)),
                   launch_rmsnorm_fp8<bf16>((const bf16*)x, x_stride, nullptr, 0, (const bf16*)w, nullptr, (uint8_t*)out, scales, rows, cols, eps, zero_centered != 0, clip, round_t != 0, S(stream)));
@@ -150,6 +161,7 @@ int dcd_k_rmsnorm_fp8(const void* x, size_t x_stride, const void* w, void* out, 
 int dcd_k_add_rmsnorm_fp8(const void* x, size_t x_stride, const void* mix, size_t mix_stride, const void* w, void* residual, void* out, float* scales, int rows,
                           int cols, float eps, int zero_centered, float clip, int round_t, int dtype, void* stream) {
   if (rows < 0 || cols <= 0 || x_stride < (size_t)cols || mix_stride < (size_t)cols || !x || !mix || !w || !residual || !out || !scales) return DCD_E_INVALID;
+  if (!whole(element_size(dtype), {x, mix, w, residual}) || !whole(4, {scales})) return DCD_E_INVALID;
   // in place only where every element is written where it was read
   if ((residual == x && x_stride != (size_t)cols) || (residual == mix && mix_stride != (size_t)cols)) return DCD_E_INVALID;
   return DISPATCH(dtype,
@@ -306,6 +318,7 @@ int dcd_k_kv4_write(const void* k, size_t k_stride, const void* v, size_t v_stri
                     void* v_scales, size_t cache_rows, int rows, int kv, int hd, int dtype, int* err, void* stream) {
   if (rows < 0 || kv <= 0 || !kv4_head_dim_ok(hd) || k_stride < (size_t)kv * hd || v_stride < (size_t)kv * hd) return DCD_E_INVALID;
   if (!k || !v || !cache_ok(k_codes, k_scales, v_codes, v_scales) || (!slots && (size_t)rows > cache_rows)) return DCD_E_INVALID;
+  if (!whole(element_size(dtype), {k, v}) || !whole(8, {slots}) || !whole(4, {err})) return DCD_E_INVALID;
   return DISPATCH(dtype,
                   launch_kv4_write<float>((const float*)k, k_stride, (const float*)v, v_stride, slots, (uint8_t*)k_codes, (uint8_t*)k_scales, (uint8_t*)v_codes, (uint8_t*)v_scales, cache_rows, rows, kv, hd, err, S(stream)),
                   launch_kv4_write<bf16>((const bf16*)k, k_stride, (const bf16*)v, v_stride, slots, (uint8_t*)k_codes, (uint8_t*)k_scales, (uint8_t*)v_codes, (uint8_t*)v_scales, cache_rows, rows, kv, hd, err, S(stream)));
@@ -315,6 +328,7 @@ int dcd_k_kv4_read(const void* k_codes, const void* k_scales, const void* v_code
                    void* v, int rows, int kv, int hd, int dtype, int* err, void* stream) {
   if (rows < 0 || kv <= 0 || !kv4_head_dim_ok(hd) || !k || !v || (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 != 0) return DCD_E_INVALID;
   if (!cache_ok(k_codes, k_scales, v_codes, v_scales) || (!slots && (size_t)rows > cache_rows)) return DCD_E_INVALID;
+  if (!whole(8, {slots}) || !whole(4, {err})) return DCD_E_INVALID;
   const Kv4Cache c = cache_of(k_codes, k_scales, v_codes, v_scales);
   return DISPATCH(dtype, launch_kv4_read<float>(c, cache_rows, slots, (float*)k, (float*)v, rows, kv, hd, err, S(stream)),
                   launch_kv4_read<bf16>(c, cache_rows, slots, (bf16*)k, (bf16*)v, rows, kv, hd, err, S(stream)));
@@ -333,6 +347,7 @@ int dcd_k_attention_kv4(const void* q, size_t q_stride, const void* k_own, size_
   if (!rows_ok(q, q_stride, (size_t)heads * hd) || !rows_ok(k_own, k_stride, (size_t)kv * hd) || !rows_ok(v_own, v_stride, (size_t)kv * hd)) return DCD_E_INVALID;
   if ((n_state > 0 && !cache_ok(k_codes, k_scales, v_codes, v_scales)) || (gate_qg && (!rows_ok(gate_qg, qg_stride, (size_t)2 * heads * hd) || qg_stride > (1u << 24)))) return DCD_E_INVALID;
   if (!out || reinterpret_cast<uintptr_t>(out) % 16 != 0 || !cu_seqlens) return DCD_E_INVALID;
+  if (!whole(4, {cu_seqlens, err})) return DCD_E_INVALID;
   const size_t need = kv4_question_workspace(B, T, n_state, heads, kv, hd);
   if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)) return DCD_E_INVALID;
   Kv4QuestionArgs a{(const bf16*)q, (const bf16*)k_own, (const bf16*)v_own, (const bf16*)gate_qg, q_stride, k_stride, v_stride, qg_stride,
@@ -352,6 +367,7 @@ int dcd_k_attention_kv4_decode(const void* q, size_t q_stride, const void* k_cod
   if (B <= 0 || T <= 0 || max_len < 0 || max_len > (1 << 30) || !heads_ok(heads, kv, hd) || !rows_ok(q, q_stride, (size_t)heads * hd)) return DCD_E_INVALID;
   if (!cache_ok(k_codes, k_scales, v_codes, v_scales) || !seg_start || !seg_len || (gate_qg && (!rows_ok(gate_qg, qg_stride, (size_t)2 * heads * hd) || qg_stride > (1u << 24)))) return DCD_E_INVALID;
   if (!out || reinterpret_cast<uintptr_t>(out) % 16 != 0 || !cu_seqlens) return DCD_E_INVALID;
+  if (!whole(4, {cu_seqlens, seg_len, err}) || !whole(8, {seg_start})) return DCD_E_INVALID;
   const size_t need = kv4_decode_workspace(B, T, max_len, heads, kv, hd);
   if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)) return DCD_E_INVALID;
   Kv4DecodeArgs a{(const bf16*)q, (const bf16*)gate_qg, q_stride, qg_stride, cache_of(k_codes, k_scales, v_codes, v_scales), cache_rows, seg_start, seg_len,

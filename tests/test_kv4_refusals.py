@@ -76,3 +76,20 @@ def test_attention_refusals(dcd):
         # no size for a shape that the call refuses
         for bad in ((0, 9, 100, 8, 2, 128), (2, 0, 100, 8, 2, 128), (2, 9, -1, 8, 2, 128), (2, 9, 100, 7, 2, 128), (2, 9, 100, 8, 2, 96)):
             assert size(*bad) == 0
+
+
+def test_pointers_off_their_elements_are_refused(dcd):
+    """On the device they would be misaligned addresses. Each operand two bytes off, or one (bf16), or four (64-bit integers)."""
+    def off(n):
+        return C.c_void_p(0x10000 + n)
+
+    for dtype, step in ((0, 2), (0, 1), (1, 1)):
+        for base, name, keys in ((NORM, "dcd_k_rmsnorm_fp8", "x w"), (ADD, "dcd_k_add_rmsnorm_fp8", "x mix w res"), (WRITE, "dcd_k_kv4_write", "k v")):
+            for key, args in with_each({**base, "dtype": dtype}, [(key, off(step)) for key in keys.split()]):
+                assert refused(dcd, name, args), (name, key)
+    for base, name, keys in ((NORM, "dcd_k_rmsnorm_fp8", "scales"), (ADD, "dcd_k_add_rmsnorm_fp8", "scales"), (WRITE, "dcd_k_kv4_write", "err slots"),
+                             (READ, "dcd_k_kv4_read", "err slots"), (QUESTIONS, "dcd_k_attention_kv4", "cu err"), (DECODE, "dcd_k_attention_kv4_decode", "cu len start err")):
+        for key, args in with_each(base, [(key, off(2)) for key in keys.split()]):
+            assert refused(dcd, name, args), (name, key)
+    for base, name, key in ((WRITE, "dcd_k_kv4_write", "slots"), (READ, "dcd_k_kv4_read", "slots"), (DECODE, "dcd_k_attention_kv4_decode", "start")):
+        assert refused(dcd, name, list({**base, key: off(4)}.values())), (name, key)
