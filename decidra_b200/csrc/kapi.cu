@@ -151,7 +151,9 @@ int dcd_k_add_rmsnorm(const void* x, const void* mix, const void* w, void* resid
 
 int dcd_k_rmsnorm_fp8(const void* x, size_t x_stride, const void* w, void* out, float* scales, int rows, int cols, float eps, int zero_centered, float clip,
                       int round_t, int dtype, void* stream) {
-  if (rows < 0 || cols <= 0 || x_stride < (size_t)cols || !x || !w || !out || !scales) return DCD_E_INVALID;
+  if (rows < 0 || cols <= 0 || x_stride < (size_t)cols || (dtype != 0 && dtype != 1)) return DCD_E_INVALID;
+  if (rows == 0) return DCD_OK;  // empty arrays have no address
+  if (!x || !w || !out || !scales) return DCD_E_INVALID;
   if (!whole(element_size(dtype), {x, w}) || !whole(4, {scales})) return DCD_E_INVALID;
   return DISPATCH(dtype,
                   launch_rmsnorm_fp8<float>((const float*)x, x_stride, nullptr, 0, (const float*)w, nullptr, (uint8_t*)out, scales, rows, cols, eps, zero_centered != 0, clip, round_t != 0, S(stream)),
@@ -160,7 +162,9 @@ int dcd_k_rmsnorm_fp8(const void* x, size_t x_stride, const void* w, void* out, 
 
 int dcd_k_add_rmsnorm_fp8(const void* x, size_t x_stride, const void* mix, size_t mix_stride, const void* w, void* residual, void* out, float* scales, int rows,
                           int cols, float eps, int zero_centered, float clip, int round_t, int dtype, void* stream) {
-  if (rows < 0 || cols <= 0 || x_stride < (size_t)cols || mix_stride < (size_t)cols || !x || !mix || !w || !residual || !out || !scales) return DCD_E_INVALID;
+  if (rows < 0 || cols <= 0 || x_stride < (size_t)cols || mix_stride < (size_t)cols || (dtype != 0 && dtype != 1)) return DCD_E_INVALID;
+  if (rows == 0) return DCD_OK;
+  if (!x || !mix || !w || !residual || !out || !scales) return DCD_E_INVALID;
   if (!whole(element_size(dtype), {x, mix, w, residual}) || !whole(4, {scales})) return DCD_E_INVALID;
   // in place only where every element is written where it was read
   if ((residual == x && x_stride != (size_t)cols) || (residual == mix && mix_stride != (size_t)cols)) return DCD_E_INVALID;
@@ -316,7 +320,8 @@ inline Kv4Cache cache_of(const void* kc, const void* ks, const void* vc, const v
 
 int dcd_k_kv4_write(const void* k, size_t k_stride, const void* v, size_t v_stride, const int64_t* slots, void* k_codes, void* k_scales, void* v_codes,
                     void* v_scales, size_t cache_rows, int rows, int kv, int hd, int dtype, int* err, void* stream) {
-  if (rows < 0 || kv <= 0 || !kv4_head_dim_ok(hd) || k_stride < (size_t)kv * hd || v_stride < (size_t)kv * hd) return DCD_E_INVALID;
+  if (rows < 0 || kv <= 0 || !kv4_head_dim_ok(hd) || k_stride < (size_t)kv * hd || v_stride < (size_t)kv * hd || (dtype != 0 && dtype != 1)) return DCD_E_INVALID;
+  if (rows == 0) return DCD_OK;
   if (!k || !v || !cache_ok(k_codes, k_scales, v_codes, v_scales) || (!slots && (size_t)rows > cache_rows)) return DCD_E_INVALID;
   if (!whole(element_size(dtype), {k, v}) || !whole(8, {slots}) || !whole(4, {err})) return DCD_E_INVALID;
   return DISPATCH(dtype,
@@ -326,7 +331,9 @@ int dcd_k_kv4_write(const void* k, size_t k_stride, const void* v, size_t v_stri
 
 int dcd_k_kv4_read(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, size_t cache_rows, const int64_t* slots, void* k,
                    void* v, int rows, int kv, int hd, int dtype, int* err, void* stream) {
-  if (rows < 0 || kv <= 0 || !kv4_head_dim_ok(hd) || !k || !v || (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 != 0) return DCD_E_INVALID;
+  if (rows < 0 || kv <= 0 || !kv4_head_dim_ok(hd) || (dtype != 0 && dtype != 1)) return DCD_E_INVALID;
+  if (rows == 0) return DCD_OK;
+  if (!k || !v || (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 != 0) return DCD_E_INVALID;
   if (!cache_ok(k_codes, k_scales, v_codes, v_scales) || (!slots && (size_t)rows > cache_rows)) return DCD_E_INVALID;
   if (!whole(8, {slots}) || !whole(4, {err})) return DCD_E_INVALID;
   const Kv4Cache c = cache_of(k_codes, k_scales, v_codes, v_scales);

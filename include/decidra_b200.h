@@ -562,7 +562,8 @@ DCD_API int dcd_k_add_rmsnorm(const void* x, const void* mix, const void* w, voi
  * x and mix are T with row strides in elements; residual may be x or mix itself where that one's stride is cols, and overlaps them in
  * no other way. round_t != 0 rounds y to T before it is quantised: the bits of dcd_k_rmsnorm / dcd_k_add_rmsnorm (zero_centered 1)
  * followed by dcd_k_quant_fp8_rows. round_t 0: y stays in f32 and is rounded once. Any cols; fastest where cols and the strides are
- * multiples of 8 (bf16) or 4 (f32) and the pointers 16-byte aligned. rows 0 does nothing. */
+ * multiples of 8 (bf16) or 4 (f32) and the pointers 16-byte aligned. rows 0 does nothing
+ * (its arrays may be NULL). */
 DCD_API int dcd_k_rmsnorm_fp8(const void* x, size_t x_stride, const void* w, void* out, float* scales, int rows, int cols, float eps, int zero_centered,
                               float clip, int round_t, int dtype, void* stream);
 DCD_API int dcd_k_add_rmsnorm_fp8(const void* x, size_t x_stride, const void* mix, size_t mix_stride, const void* w, void* residual, void* out,
@@ -676,7 +677,7 @@ DCD_API int dcd_k_attention_tc_noalloc(const void* q, const void* k_own, int k_s
  * write: token i's K and V (T rows with strides in elements) go to cache row slots[i]; slots == NULL: row i. A negative slot leaves
  * its token out; a slot >= cache_rows sets *err and is left out. The slots of one call are distinct.
  * read: cache row slots[i] (or i) to row i of k and v, [rows, kv, hd] T, 16-byte aligned; code * scale is exact in T. Rows of
- * negative or bad slots are left as they were. rows 0 does nothing; err may be NULL. */
+ * negative or bad slots are left as they were. rows 0 does nothing (the arrays may then be NULL); err may be NULL. */
 DCD_API int dcd_k_kv4_write(const void* k, size_t k_stride, const void* v, size_t v_stride, const int64_t* slots, void* k_codes, void* k_scales,
                             void* v_codes, void* v_scales, size_t cache_rows, int rows, int kv, int hd, int dtype, int* err, void* stream);
 DCD_API int dcd_k_kv4_read(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, size_t cache_rows, const int64_t* slots,

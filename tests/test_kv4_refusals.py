@@ -93,3 +93,13 @@ def test_pointers_off_their_elements_are_refused(dcd):
             assert refused(dcd, name, args), (name, key)
     for base, name, key in ((WRITE, "dcd_k_kv4_write", "slots"), (READ, "dcd_k_kv4_read", "slots"), (DECODE, "dcd_k_attention_kv4_decode", "start")):
         assert refused(dcd, name, list({**base, key: off(4)}.values())), (name, key)
+
+
+def test_no_rows_need_no_arrays(dcd):
+    """Arrays of no elements have no address: rows 0 does nothing and succeeds, whatever the sizes that are checked allow."""
+    from decidra_b200 import _lib
+    for base, name, arrays in ((NORM, "dcd_k_rmsnorm_fp8", "x out scales"), (ADD, "dcd_k_add_rmsnorm_fp8", "x mix res out scales"), (WRITE, "dcd_k_kv4_write", "k v"),
+                               (READ, "dcd_k_kv4_read", "k v"), (WRITE, "dcd_k_kv4_write", "k v kc ksc vc vsc"), (READ, "dcd_k_kv4_read", "k v kc ksc vc vsc")):
+        args = {**base, "rows": 0, **{key: None for key in arrays.split()}}
+        assert getattr(_lib.load(), name)(*args.values()) == 0, name
+        assert refused(dcd, name, list({**args, "dtype": 2}.values())), name
