@@ -710,7 +710,8 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       if (n_tiles == 1 && live > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar_o_free, (uint32_t)(live - 1) & 1, abort_flag));
     }
     if (ok) {
-      l_part[h * 128 + r] = m == -INFINITY ? 0.f : l * ex2(m - end_m);
+      // a group that has seen no score: m = -inf and l = 0, or NaN where all of its scores were, which the sum has to show
+      l_part[h * 128 + r] = m == -INFINITY ? l : l * ex2(m - end_m);
       mbar_arrive(bar_l);
       ok = __all_sync(0xffffffffu, mbar_wait(bar_l, (uint32_t)live & 1, abort_flag));
     }
@@ -720,7 +721,7 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       tc_fence_after();
       const float sum = l_part[r] + l_part[128 + r];
       if (p.parts > 1 && h == 0) p.ws_ml[block_lin * 128 + r] = make_float2(end_m, sum);
-      const float inv = p.parts > 1 ? 1.0f : sum > 0.f ? 1.0f / sum : 0.f;
+      const float inv = p.parts > 1 ? 1.0f : sum == 0.f ? 0.f : 1.0f / sum;
       uint8_t* stage = smem + D::Q_BYTES + e_slot * SLOT + warp * (SLOT / 8);
       auto swz = [](int row) { return CH == 32 ? row & 7 : (row >> 1) & 3; };  // 16-byte chunks of a row: no two lanes of a quarter in one bank
 #pragma unroll 1
@@ -815,7 +816,7 @@ __global__ void __launch_bounds__(128) kv4_attention_merge_kernel(const Params p
   for (int k = 0; k < 4; ++k) {
     const int z = lane + 32 * k;
     ml[k] = z < parts ? p.ws_ml[z * step + row0] : make_float2(-INFINITY, 0.f);
-    if (ml[k].y > 0.f) M = fmaxf(M, ml[k].x);
+    M = fmaxf(M, ml[k].x);
   }
   M = warp_max(M);
   float acc[PER], sum = 0.f;
@@ -824,10 +825,12 @@ __global__ void __launch_bounds__(128) kv4_attention_merge_kernel(const Params p
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     if (32 * k >= parts) break;
-    // a part without keys, or one that this row sees nothing of, may have written no O: weight 0, and its row is not read
-    const float wt = ml[k].y > 0.f ? ex2(ml[k].x - M) : 0.f;
+    // a part without keys, or one that this row sees nothing of, may have written no O: its sum is 0, and its row is not read. A sum of
+    // NaN is none of these: it and its row count, at a weight of 0 too, so that a question whose keys are split shows a NaN as any other
+    const bool some = ml[k].y != 0.f;
+    const float wt = some ? ex2(ml[k].x - M) : 0.f;
     sum += wt * ml[k].y;
-    const uint32_t have = __ballot_sync(0xffffffffu, wt > 0.f);
+    const uint32_t have = __ballot_sync(0xffffffffu, some);
     const float* src = p.ws_o + (32 * k * step + row0) * HD + lane * PER;
     for (int z0 = 0; z0 < 32 && 32 * k + z0 < parts; z0 += U) {  // U rows are asked for before the first is used
       float2 v[U][PER / 2];
@@ -849,7 +852,7 @@ __global__ void __launch_bounds__(128) kv4_attention_merge_kernel(const Params p
   }
   sum = warp_sum(sum);
   const size_t t = (size_t)found[0] + found[1] + tt;
-  const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   const bf16* gate = p.gate_qg ? p.gate_qg + t * p.qg_stride + (size_t)(2 * head + 1) * HD + lane * PER : nullptr;
   bf16* dst = p.out + (t * p.heads + head) * HD + lane * PER;
 #pragma unroll

@@ -2,7 +2,7 @@
 in calls whose keys are split, loose bounds, offsets that fall, operands off their alignment, and every key counted once."""
 import pytest
 
-from test_gpu_kv4 import Questions
+from test_gpu_kv4 import Questions, attend, values
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,58 @@ def test_items_of_one_key_tile_behind_each_other(G, hd, causal):
         c.launch(G)
         torch.cuda.synchronize()
         assert torch.equal(first, c.out)
+
+
+# ---------------------------------------------------------------------------------------------
+# values that are not finite
+# ---------------------------------------------------------------------------------------------
+NAN, INF = float("nan"), float("inf")
+
+
+def near(got, want, spread):
+    """The bound of test_gpu_kv4.close, where the value is finite."""
+    off = (got.double() - want).abs()
+    assert (off <= 2.0 ** -8 * want.abs() + (2.0 ** -7 + 1e-3) * spread + 1e-30).all()
+
+
+@pytest.mark.parametrize("heads,kv,hd", [(24, 4, 256), (16, 2, 128), (4, 1, 64)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("where", ["query", "query inf", "own key", "every own key", "state key", "own value", "state value"])
+def test_questions_show_a_nan_whether_their_keys_are_split_or_not(G, heads, kv, hd, causal, where):
+    """One question over a long state has its keys split into parts, the same one among a hundred others has not: a NaN shows in the rows
+    that see it, in both, and nowhere else."""
+    import torch
+    n, S, kh, rep = 16, 4000, kv - 1, heads // kv
+    for others in (0, 160):
+        c = Questions([n] + [20] * others, S, heads, kv, hd, causal, False)
+        ks, vs = values(*c.cache[:2])[:S], values(*c.cache[2:])[:S]
+        seen = torch.ones(n, S + n, dtype=torch.bool, device="cuda")
+        if causal:
+            seen[:, S:] = seen[:, S:].tril()
+        want, spread = attend(c.q[:n], torch.cat((ks, c.k[:n].double().reshape(n, kv, hd))), torch.cat((vs, c.v[:n].double().reshape(n, kv, hd))), seen)
+        bad = torch.zeros(n, heads, hd, dtype=torch.bool, device="cuda")
+        group = slice(kh * rep, (kh + 1) * rep)
+        if where.startswith("query"):
+            c.q[5, 1, 7] = INF if where.endswith("inf") else NAN  # infinite scores of either sign: NaN as well
+            bad[5, 1] = True
+        elif where == "own key":
+            c.k[6, kh * hd + 3] = NAN
+            bad[6 if causal else 0:, group] = True
+        elif where == "every own key":
+            c.k[:n, kh * hd + 3] = NAN
+            bad[:, group] = True
+        elif where == "state key":
+            c.cache[1][1234, kh, 0] = 0x7F
+            bad[:, group] = True
+        elif where == "own value":
+            c.v[0, kh * hd + 3] = NAN
+            bad[:, group, 3] = True
+        else:
+            c.cache[3][1234, kh, 1] = 0x7F
+            bad[:, group, 16:32] = True
+        c.launch(G)
+        torch.cuda.synchronize()
+        assert int(c.err.item()) == 0
+        got = c.out[:n]
+        assert torch.equal(torch.isnan(got), bad)
+        near(got[~bad], want[~bad], spread[~bad])
