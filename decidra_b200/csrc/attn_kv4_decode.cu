@@ -151,7 +151,7 @@ __device__ __forceinline__ int blocks_of(const Sequence& s) { return max(1, (s.l
 // PER consecutive values of a row from dimension d: normalised, gated, rounded once; stored N at a time
 template <int PER>
 __device__ __forceinline__ void store_row(const Kv4DecodeArgs& a, const float (&acc)[PER], float sum, size_t at, int t, int h, int hd, int d) {
-  const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // 0: a token that sees no row; NaN stays
   const bf16* gate = a.gate_qg ? a.gate_qg + (size_t)t * a.qg_stride + (size_t)(2 * h + 1) * hd + d : nullptr;
   bf16* out = a.out + at * hd + d;
   constexpr int N = PER < 8 ? PER : 8;
@@ -614,12 +614,13 @@ __global__ void __launch_bounds__(W > 4 ? W * 32 : 128) kv4_decode_merge_kernel(
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) acc[i][j] = 0.f;
-  if (nz > 1 && M != -INFINITY) {
+  if (nz > 1) {
     const float* src = p.ws_o + at * p.max_parts * HD + lane * VEC;
     for (int z0 = w; z0 < nz; z0 += 32 * W) {  // this warp's next 32 parts: z0, z0 + W, ...
       const int mine = z0 + lane * W;
       const float2 x = mine < nz ? ml[mine] : make_float2(-INFINITY, 0.f);
-      const float wt = ex2(x.x - M);  // a part that saw nothing has m = -inf: weight 0 on zeros
+      // a part that saw nothing has m = -inf and sum 0: weight 0 on zeros. One whose scores are all NaN has m = -inf and sum NaN, which stays
+      const float wt = x.y == 0.f ? 0.f : ex2(x.x - M);
       sum += wt * x.y;
       const int n = min(32, (nz - z0 + W - 1) / W);
       for (int z = 0; z < n; z += U) {

@@ -2,7 +2,7 @@
 in calls whose keys are split, loose bounds, offsets that fall, operands off their alignment, and every key counted once."""
 import pytest
 
-from test_gpu_kv4 import Questions, attend, values
+from test_gpu_kv4 import Decode, Questions, attend, values
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +89,40 @@ def test_questions_show_a_nan_whether_their_keys_are_split_or_not(G, heads, kv, 
         got = c.out[:n]
         assert torch.equal(torch.isnan(got), bad)
         near(got[~bad], want[~bad], spread[~bad])
+
+
+@pytest.mark.parametrize("heads,kv,hd", [(24, 4, 256), (16, 2, 128), (4, 1, 64), (16, 4, 128)])
+@pytest.mark.parametrize("where", ["query", "query inf", "key", "every key", "value"])
+def test_new_tokens_show_a_nan_whether_their_keys_are_split_or_not(G, heads, kv, hd, where):
+    """The same in the form for new tokens: three drafted tokens over a stretch that one warp takes, over one of many parts, and beside one
+    that is too short for the first two (they see no row and give 0, whatever they ask)."""
+    import torch
+    L, kh, rep = 3, kv - 1, heads // kv
+    for n in (20, 6000):
+        c = Decode([n, 1], L, heads, kv, hd)
+        s, s1 = c.start
+        k, v = values(*c.cache[:2]), values(*c.cache[2:])
+        seen = torch.arange(n, device="cuda")[None] <= (n - L + torch.arange(L, device="cuda"))[:, None]
+        want, spread = attend(c.q[:L].reshape(L, heads, hd), k[s:s + n], v[s:s + n], seen)
+        bad = torch.zeros(L, heads, hd, dtype=torch.bool, device="cuda")
+        group = slice(kh * rep, (kh + 1) * rep)
+        if where.startswith("query"):
+            c.q[1, hd + 7] = INF if where.endswith("inf") else NAN
+            bad[1, 1] = True
+            c.q[L:L + 2] = NAN
+        elif where == "key":
+            c.cache[1][s + n - 2, kh, 0] = 0x7F  # the first token does not see it
+            bad[1:, group] = True
+        elif where == "every key":
+            c.cache[1][s:s + n, kh, 0] = 0x7F
+            bad[:, group] = True
+        else:
+            c.cache[3][s + 7, kh, 1] = 0x7F
+            bad[:, group, 16:32] = True
+        c.launch(G)
+        torch.cuda.synchronize()
+        assert int(c.err.item()) == 0
+        got = c.out[:L]
+        assert torch.equal(torch.isnan(got), bad)
+        near(got[~bad], want[~bad], spread[~bad])
+        assert (c.out[L:L + 2] == 0).all() and (c.out[2 * L:] == -7.0).all()
