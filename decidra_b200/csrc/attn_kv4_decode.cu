@@ -40,8 +40,9 @@ constexpr float P_SHIFT = 10.0f;  // P is held as p * 2^10
 
 constexpr int WARPS = 4;
 // CTAs per SM, Q fragments in shared memory where registers run out
+constexpr int ctas_of(int nt) { return nt == 1 ? 3 : 2; }
 template <int HD, int NT> struct Cfg {
-  static constexpr int CTAS = NT == 1 ? 3 : 2;
+  static constexpr int CTAS = ctas_of(NT);
   static constexpr bool Q_SMEM = NT * HD >= 256;
 };
 
@@ -109,11 +110,17 @@ struct Args {
   Kv4DecodeArgs a;
   int hc;          // K/V heads of a pair: 4, 2 or 1
   int q_min;       // least blocks per CTA
-  int max_parts;   // parts of a row, at most: max_len in blocks / q_min, and one more for its offset, times the warps of a head
-  float* ws_o;     // [T * heads][max_parts][hd]
-  float2* ws_ml;   // [T * heads][max_parts] (maximum in log2 units, sum)
-  int* ws_n;       // [T * heads] parts of the row's pair
+  uint32_t split;  // places of pairs that are split between CTAs; the others' are behind them
+  float* ws_o;     // [places][hd] unnormalised O of a part of a row
+  float2* ws_ml;   // [places] (maximum in log2 units, sum)
+  uint2* ws_n;     // [T * heads] the row's parts and the place of its first: they lie behind each other
 };
+
+// The first place of a row of a pair that is split between CTAs from `first_cta` on. A warp's row has a place for every even number of a CTA
+// and every odd one: the parts of a pair go to 2 first_cta and the numbers behind it, and the next pair that is split begins in the last CTA
+// of this one or later, so that twice its number is above all of them. That bounds the places by the CTAs, whatever the lengths are and however many
+// parts a row has.
+__device__ __forceinline__ uint32_t split_place(int row, int first_cta, int step) { return ((uint32_t)row * gridDim.x + first_cta) * (2 * step); }
 
 struct Sequence {
   int off, L, len;
@@ -554,10 +561,11 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<HD, NT>::CTAS) kv4_decode_kern
         if (r >= n_rows) continue;
         const int tt = r / G, tok = sq.off + tt, h = kh * G + r - tt * G;
         const size_t at = (size_t)tok * a.heads + h;
-        if (my_part == 0 && g == 0) p.ws_n[at] = parts_all;
+        const uint32_t base = n_parts == 1 ? p.split + (uint32_t)at * step : split_place(my_head * ROWS + r - r0, first_cta, step);
+        if (my_part == 0 && g == 0) p.ws_n[at] = make_uint2(parts_all, base);
         if (parts_all > 1) {
-          if (g == 0) p.ws_ml[at * p.max_parts + my_part] = make_float2(m[nt][i], l[nt][i]);
-          float* dst = p.ws_o + (at * p.max_parts + my_part) * HD + g * (HD / 8);
+          if (g == 0) p.ws_ml[base + my_part] = make_float2(m[nt][i], l[nt][i]);
+          float* dst = p.ws_o + (size_t)(base + my_part) * HD + g * (HD / 8);
 #pragma unroll
           for (int t = 0; t < HD / 16; t += 2)
             *reinterpret_cast<float4*>(dst + 2 * t) = make_float4(o[t][nt][i], o[t][nt][i + 2], o[t + 1][nt][i], o[t + 1][nt][i + 2]);
@@ -591,6 +599,7 @@ __global__ void __launch_bounds__(W > 4 ? W * 32 : 128) kv4_decode_merge_kernel(
   const size_t at = (size_t)blockIdx.x * (WARPS_HERE / W) + warp / W;
   const int t = (int)(at / (unsigned)a.heads), h = (int)(at - (size_t)t * a.heads);
   int nz = 0;
+  size_t base = 0;
   if (t < a.T) {
     int lo = 0, hi = a.B;  // cu[lo] <= t, and t < cu[hi] where it is in a sequence at all
     while (hi - lo > 1) {
@@ -601,10 +610,14 @@ __global__ void __launch_bounds__(W > 4 ? W * 32 : 128) kv4_decode_merge_kernel(
       lo += n * step;
     }
     const int off = a.cu[lo], end = a.cu[lo + 1];
-    if (off >= 0 && off <= t && t < end && end <= a.T) nz = p.ws_n[at];
+    if (off >= 0 && off <= t && t < end && end <= a.T) {
+      const uint2 n = p.ws_n[at];
+      nz = (int)n.x;
+      base = n.y;
+    }
   }
   if (W == 1 && nz <= 1) return;  // finished by its only warp, or no token of a sequence
-  const float2* ml = p.ws_ml + at * p.max_parts;
+  const float2* ml = p.ws_ml + base;
   float M = -INFINITY;
 #pragma unroll 4
   for (int z = lane; z < nz; z += 32) M = fmaxf(M, ml[z].x);
@@ -615,7 +628,7 @@ __global__ void __launch_bounds__(W > 4 ? W * 32 : 128) kv4_decode_merge_kernel(
 #pragma unroll
     for (int j = 0; j < VEC; ++j) acc[i][j] = 0.f;
   if (nz > 1) {
-    const float* src = p.ws_o + at * p.max_parts * HD + lane * VEC;
+    const float* src = p.ws_o + base * HD + lane * VEC;
     for (int z0 = w; z0 < nz; z0 += 32 * W) {  // this warp's next 32 parts: z0, z0 + W, ...
       const int mine = z0 + lane * W;
       const float2 x = mine < nz ? ml[mine] : make_float2(-INFINITY, 0.f);
@@ -680,34 +693,47 @@ int sm_count() {
   return sms;
 }
 
-// The K/V heads of a pair, the SMs, the least blocks that a CTA takes (two per warp, and not so few that the parts of a pair outgrow the
-// workspace where most sequences are far shorter than max_len), and the parts that a pair can then have.
+// How a call is cut up. The blocks per CTA follow the lengths on the device: max_len only bounds the CTAs and parts of a small call, so that
+// a bound far above the lengths costs neither time nor memory. (With a least share that grew with B * max_len, 64 sequences of about 1000
+// rows took 393 us under a bound of 131072, where they take 35 under any, and one of 100000 rows among 199 short ones 1215, now 89.)
 struct Plan {
-  int hc, sms, q_min, max_parts;
+  int hc, nt, grid, q_min;  // K/V heads of a pair, column tiles of eight rows, CTAs, least blocks per CTA
+  int parts;                // of a row, where the sequences are about as long as each other
+  size_t split, places;     // places of parts: of the pairs split between CTAs, and all
 };
-Plan plan_of(int B, int kv, int max_len) {
+Plan plan_of(int B, int T, int max_len, int heads, int kv, int hd) {
   Plan p;
   p.hc = kv % 4 == 0 ? 4 : kv % 2 == 0 ? 2 : 1;
-  p.sms = sm_count();
-  const long long blocks = max(1LL, ((long long)max_len + KB - 1) / KB);
-  const double share = (double)B * (kv / p.hc) * (double)blocks / (8.0 * p.sms);  // an eighth of what the CTAs of two per SM would take
-  p.q_min = (int)max(2LL * WARPS / p.hc, (long long)min(ceil(share), (double)blocks));
-  p.max_parts = (int)((blocks + p.q_min - 1) / p.q_min + 1) * (WARPS / p.hc);
+  // column tiles by the rows of a sequence of average length; longer ones take several rounds over their keys
+  const long long rows = ((long long)T + B - 1) / B * (heads / kv);
+  p.nt = rows <= 8 ? 1 : rows <= 16 || hd == 256 ? 2 : 4;
+  const int sms = sm_count(), wave = sms * ctas_of(p.nt), step = WARPS / p.hc;
+  p.q_min = 2 * step;  // two per warp
+  const long long pairs = (kv / p.hc) * ((long long)T * (heads / kv) / (8 * p.nt) + B), blocks = max(1LL, ((long long)max_len + KB - 1) / KB);
+  p.grid = (double)pairs * (double)blocks >= (double)wave * p.q_min ? wave : (int)((pairs * blocks + p.q_min - 1) / p.q_min);
+  p.parts = (int)min((blocks + p.q_min - 1) / p.q_min + 1, p.grid / pairs + 2) * step;
+  // no more with more tokens, sequences or rows than the workspace of the largest call holds: sized for the column tiles that a call of the same
+  // heads may take at most (grid * nt <= units)
+  const int nt_max = hd == 256 ? 2 : 4;
+  const double units = (kv / p.hc) * ((double)T * (heads / kv) / 8 + (double)B * nt_max) * (double)blocks / p.q_min + nt_max;
+  p.split = (size_t)2 * WARPS * 8 * (size_t)min(ceil(units), (double)sms * ctas_of(nt_max) * nt_max);
+  p.places = p.split + (step > 1 ? (size_t)T * heads * step : 0);
   return p;
 }
 
 template <int HD, int NT>
-cudaError_t run(const Args& p, int sms, cudaStream_t s) {
+cudaError_t run(const Args& p, const Plan& plan, cudaStream_t s) {
   using C = Cfg<HD, NT>;
   constexpr int bytes = WARPS * (Block<HD>::BYTES + (C::Q_SMEM ? HD / 16 * NT * 256 : 0));
   static_assert(C::CTAS * (bytes + 1024 + 256) <= 228 * 1024, "shared memory of an SM");
   CUDA_TRY(cudaFuncSetAttribute(kv4_decode_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  kv4_decode_kernel<HD, NT><<<sms * C::CTAS, WARPS * 32, bytes, s>>>(p);
+  kv4_decode_kernel<HD, NT><<<plan.grid, WARPS * 32, bytes, s>>>(p);
   CUDA_TRY(cudaGetLastError());
   const size_t rows = (size_t)p.a.T * p.a.heads;
-  // more warps a row where more parts make a longer chain; fewer where they would have less than a part or two each
-  if (p.max_parts <= 8) kv4_decode_merge_kernel<HD, 1><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
-  else if (p.max_parts <= 32) kv4_decode_merge_kernel<HD, 4><<<(unsigned)rows, 128, 0, s>>>(p);
+  // More warps a row where more parts make a longer chain; fewer where they would have less than a part or two each (256 sequences of
+  // about 1000 rows, most of them of one part: 83 us with a warp a row, 94 with four; one of 100000 among 199 short ones 89 and 69)
+  if (plan.parts <= 8) kv4_decode_merge_kernel<HD, 1><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
+  else if (plan.parts <= 32) kv4_decode_merge_kernel<HD, 4><<<(unsigned)rows, 128, 0, s>>>(p);
   else kv4_decode_merge_kernel<HD, 16><<<(unsigned)rows, 512, 0, s>>>(p);
   return cudaGetLastError();
 }
@@ -715,25 +741,22 @@ cudaError_t run(const Args& p, int sms, cudaStream_t s) {
 }  // namespace kvd
 
 size_t kv4_decode_workspace(int B, int T, int max_len, int heads, int kv, int hd) {
-  const size_t rows = (size_t)T * heads, parts = (size_t)kvd::plan_of(B, kv, max_len).max_parts;
-  return rows * (parts * ((size_t)hd * sizeof(float) + sizeof(float2)) + sizeof(int));
+  const kvd::Plan p = kvd::plan_of(B, T, max_len, heads, kv, hd);
+  return p.places * ((size_t)hd * sizeof(float) + sizeof(float2)) + (size_t)T * heads * sizeof(uint2);
 }
 
 cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, void* workspace, cudaStream_t s) {
-  const kvd::Plan plan = kvd::plan_of(a.B, a.kv, a.max_len);
-  const size_t parts = (size_t)a.T * a.heads * plan.max_parts;
+  const kvd::Plan plan = kvd::plan_of(a.B, a.T, a.max_len, a.heads, a.kv, a.hd);
+  if (plan.places >> 32) return cudaErrorInvalidValue;  // a workspace of a terabyte
   kvd::Args p;
   p.a = a;
   p.hc = plan.hc;
   p.q_min = plan.q_min;
-  p.max_parts = plan.max_parts;
+  p.split = (uint32_t)plan.split;
   p.ws_o = (float*)workspace;
-  p.ws_ml = (float2*)(p.ws_o + parts * a.hd);
-  p.ws_n = (int*)(p.ws_ml + parts);
-  // column tiles of eight rows by the rows of a sequence of average length; longer ones take several rounds over their keys
-  const long long rows = ((long long)a.T + a.B - 1) / a.B * (a.heads / a.kv);
-  const int n = plan.sms;
-  if (a.hd == 256) return rows <= 8 ? kvd::run<256, 1>(p, n, s) : kvd::run<256, 2>(p, n, s);
-  if (a.hd == 128) return rows <= 8 ? kvd::run<128, 1>(p, n, s) : rows <= 16 ? kvd::run<128, 2>(p, n, s) : kvd::run<128, 4>(p, n, s);
-  return rows <= 8 ? kvd::run<64, 1>(p, n, s) : rows <= 16 ? kvd::run<64, 2>(p, n, s) : kvd::run<64, 4>(p, n, s);
+  p.ws_ml = (float2*)(p.ws_o + plan.places * a.hd);
+  p.ws_n = (uint2*)(p.ws_ml + plan.places);
+  if (a.hd == 256) return plan.nt == 1 ? kvd::run<256, 1>(p, plan, s) : kvd::run<256, 2>(p, plan, s);
+  if (a.hd == 128) return plan.nt == 1 ? kvd::run<128, 1>(p, plan, s) : plan.nt == 2 ? kvd::run<128, 2>(p, plan, s) : kvd::run<128, 4>(p, plan, s);
+  return plan.nt == 1 ? kvd::run<64, 1>(p, plan, s) : plan.nt == 2 ? kvd::run<64, 2>(p, plan, s) : kvd::run<64, 4>(p, plan, s);
 }

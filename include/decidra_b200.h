@@ -699,8 +699,9 @@ DCD_API int dcd_k_attention_kv4(const void* q, size_t q_stride, const void* k_ow
 /* The form for new tokens: sequence b's rows in the cache are [seg_start[b], seg_start[b] + seg_len[b]), its packed tokens
  * [cu_seqlens[b], cu_seqlens[b + 1]) are the newest ones, already written there: the last token sees every row of the stretch, each
  * one before it a row less. Stretches may be shared or overlap. A token that sees no row (more tokens than rows) gives 0. A stretch
- * that leaves the cache or is longer than max_len sets *err, and its tokens give 0. max_len is at most 2^30 (the workspace grows with
- * it). Meant for one to a few tokens a sequence; every other operand as above. */
+ * that leaves the cache or is longer than max_len sets *err, and its tokens give 0. max_len is at most 2^30; a bound far above
+ * the lengths costs neither time nor memory (the workspace has a fixed part of up to 40 MB and, where kv is not a multiple of 4, one that
+ * grows with T * heads). Meant for one to a few tokens a sequence; every other operand as above. */
 DCD_API size_t dcd_k_attention_kv4_decode_workspace(int B, int T, int max_len, int heads, int kv, int hd);
 DCD_API int dcd_k_attention_kv4_decode(const void* q, size_t q_stride, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
                                        size_t cache_rows, const int64_t* seg_start, const int32_t* seg_len, int max_len, const void* gate_qg,

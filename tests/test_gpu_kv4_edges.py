@@ -126,3 +126,37 @@ def test_new_tokens_show_a_nan_whether_their_keys_are_split_or_not(G, heads, kv,
         assert torch.equal(torch.isnan(got), bad)
         near(got[~bad], want[~bad], spread[~bad])
         assert (c.out[L:L + 2] == 0).all() and (c.out[2 * L:] == -7.0).all()
+
+
+# ---------------------------------------------------------------------------------------------
+# the bound on the lengths
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("heads,kv,hd", [(24, 4, 256), (16, 2, 128), (4, 1, 64)])
+def test_a_loose_bound_on_the_lengths_costs_no_time(G, heads, kv, hd):
+    """64 sequences of about a thousand rows, called with their longest length and with a context limit of 131072."""
+    import torch
+    took = []
+    for bound in (None, 131072):
+        c = Decode([900 + 3 * i for i in range(64)], 1, heads, kv, hd, max_len=bound)
+        c.launch(G)
+        c.check()
+        times = []
+        for _ in range(10):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(10):
+                c.launch(G)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        took.append(sorted(times)[5])
+    assert took[1] < 2 * took[0], took
+
+
+@pytest.mark.parametrize("heads,kv,hd", [(24, 4, 256), (16, 2, 128), (4, 1, 64), (15, 3, 256)])
+@pytest.mark.parametrize("bound", [None, 1 << 30])
+def test_new_tokens_of_very_different_lengths(G, heads, kv, hd, bound):
+    """One long stretch among many short ones, whose keys then go to hundreds of parts, and sequences with more tokens than a round."""
+    c = Decode([5 + i % 90 for i in range(70)] + [40000] + [3, 0, 700], [1] * 70 + [2, 40, 1, 17], heads, kv, hd, gate=True, max_len=bound)
+    c.launch(G)
+    c.check()

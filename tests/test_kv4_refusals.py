@@ -103,3 +103,18 @@ def test_no_rows_need_no_arrays(dcd):
         args = {**base, "rows": 0, **{key: None for key in arrays.split()}}
         assert getattr(_lib.load(), name)(*args.values()) == 0, name
         assert refused(dcd, name, list({**args, "dtype": 2}.values())), name
+
+
+def test_new_tokens_workspace_is_bounded(dcd):
+    """A bound far above the lengths and many tokens of one sequence both cost next to nothing; a call of one token asks for little."""
+    from decidra_b200 import _lib
+    size = _lib.load().dcd_k_attention_kv4_decode_workspace
+    assert size(64, 64, 1 << 30, 24, 4, 256) == size(64, 64, 20000, 24, 4, 256) < 64 << 20
+    assert size(1, 2000, 100_000, 24, 4, 256) < 64 << 20
+    assert size(1, 2000, 100_000, 16, 1, 128) < 128 << 20
+    assert size(1, 1, 2048, 24, 4, 256) < 8 << 20
+    # what is enough for the largest call is enough for every smaller one
+    for heads, kv, hd in ((24, 4, 256), (16, 2, 128), (4, 1, 64), (15, 3, 256)):
+        largest = size(64, 300, 20000, heads, kv, hd)
+        for B, T, n in ((64, 64, 20000), (1, 300, 20000), (1, 1, 20000), (2, 8, 777), (64, 300, 1), (9, 36, 8192), (1, 4, 16384)):
+            assert size(B, T, n, heads, kv, hd) <= largest
