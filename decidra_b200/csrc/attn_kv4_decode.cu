@@ -609,8 +609,14 @@ __global__ void __launch_bounds__(W > 4 ? W * 32 : 128) kv4_decode_merge_kernel(
       hi = min(lo + (n + 1) * step, hi);
       lo += n * step;
     }
-    const int off = a.cu[lo], end = a.cu[lo + 1];
-    if (off >= 0 && off <= t && t < end && end <= a.T) {
+    auto has = [&](int i) {  // sequence i is sound and t one of its tokens
+      const int off = a.cu[i], end = a.cu[i + 1];
+      return off >= 0 && off <= t && t < end && end <= a.T;
+    };
+    bool mine = has(lo);
+    // not there: a row behind the last sequence, or offsets that fall, among which a sound sequence may have been missed
+    for (int i = lane; !mine && i - lane < a.B; i += 32) mine = __any_sync(0xffffffffu, i < a.B && has(i));
+    if (mine) {
       const uint2 n = p.ws_n[at];
       nz = (int)n.x;
       base = n.y;

@@ -160,3 +160,29 @@ def test_new_tokens_of_very_different_lengths(G, heads, kv, hd, bound):
     c = Decode([5 + i % 90 for i in range(70)] + [40000] + [3, 0, 700], [1] * 70 + [2, 40, 1, 17], heads, kv, hd, gate=True, max_len=bound)
     c.launch(G)
     c.check()
+
+
+# ---------------------------------------------------------------------------------------------
+# offsets
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("cu", [[0, 99, 3, 12], [5, 2 ** 31 - 1, 0, 12], [-7, 9, 2, 12], [0, 4, 99, 4, 12]])
+@pytest.mark.parametrize("heads,kv,hd", [(16, 2, 128), (24, 4, 256)])
+def test_new_tokens_of_a_sound_sequence_behind_offsets_that_fall(G, cu, heads, kv, hd):
+    """Its keys are split into parts, which have to be added up whatever the offsets in front of it are."""
+    import torch
+    n = len(cu) - 1
+    c = Decode([5000, 60, 3000, 7000][:n], [4] * n, heads, kv, hd, behind=0)
+    c.T = 12
+    c.cu.copy_(torch.tensor(cu, dtype=torch.int32))
+    c.launch(G)
+    torch.cuda.synchronize()
+    assert int(c.err.item()) == 8
+    k, v = values(*c.cache[:2]), values(*c.cache[2:])
+    taken = set()
+    for i, (a, b) in enumerate(zip(cu, cu[1:])):
+        if 0 <= a <= b <= c.T:
+            taken |= set(range(a, b))
+            s, m, L = c.start[i], c.lens[i], b - a
+            seen = torch.arange(m, device="cuda")[None] <= (m - L + torch.arange(L, device="cuda"))[:, None]
+            near(c.out[a:b], *attend(c.q[a:b].reshape(L, heads, hd), k[s:s + m], v[s:s + m], seen))
+    assert (c.out[[t for t in range(12) if t not in taken]] == -7.0).all()
