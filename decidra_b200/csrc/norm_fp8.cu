@@ -15,6 +15,8 @@
 // max|r * (w + wofs)| * inv to the bit.
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -52,10 +54,23 @@ template <typename T> struct Pack<T, 1> {
   static __device__ __forceinline__ void st(T* p, const float (&f)[1]) { Ty<T>::st(p, f[0]); }
 };
 
-template <int V>
+// The same V elements one by one, where the address forbids the access but their order is wanted
+template <typename T, int V> struct Single {
+  static __device__ __forceinline__ void ld(const T* p, float (&f)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = Ty<T>::ld(p + i);
+  }
+  static __device__ __forceinline__ void st(T* p, const float (&f)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) Ty<T>::st(p + i, f[i]);
+  }
+};
+
+template <int V, bool WIDE = V != 1>
 __device__ __forceinline__ void store_codes(uint8_t* p, const float (&f)[V]) {
-  if constexpr (V == 1) {
-    *p = (uint8_t)__nv_cvt_float_to_fp8(f[0], __NV_SATFINITE, __NV_E4M3);
+  if constexpr (!WIDE) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) p[i] = (uint8_t)__nv_cvt_float_to_fp8(f[i], __NV_SATFINITE, __NV_E4M3);
   } else {
     uint32_t w[V / 4];
 #pragma unroll
@@ -80,10 +95,11 @@ __device__ __forceinline__ void block_sum_max(float& a, float& b, float* red) {
 
 // One CTA per row, the row in registers: V * NV values a thread, cols <= V * NV * blockDim.x. x, mix and residual may be one buffer
 // (every element is read before the same thread writes it), so none of them is restrict-qualified.
-template <typename T, int V, int NV, bool ADD, bool ROUND>
+template <typename T, int V, int NV, bool ADD, bool ROUND, bool WIDE = true>
 __global__ void __launch_bounds__(ROUND ? 256 : 1024) rmsnorm_fp8_kernel(const T* x, size_t x_stride, const T* mix, size_t mix_stride, const T* __restrict__ w,
                                                            T* residual, uint8_t* __restrict__ out, float* __restrict__ scales, int cols, float eps,
                                                            float wofs, float clip) {
+  using P = std::conditional_t<WIDE, Pack<T, V>, Single<T, V>>;
   __shared__ float red[128];
   const size_t row = blockIdx.x;
   const int n = cols / V, nt = (int)blockDim.x;
@@ -94,9 +110,9 @@ __global__ void __launch_bounds__(ROUND ? 256 : 1024) rmsnorm_fp8_kernel(const T
   for (int c = 0; c < NV; ++c) {  // all loads before the first use
     const int i = (int)threadIdx.x + c * nt;
     if (i < n) {
-      Pack<T, V>::ld(xr + (size_t)i * V, v[c]);
-      if constexpr (ADD) Pack<T, V>::ld(mix + row * mix_stride + (size_t)i * V, m[c]);
-      if constexpr (!ROUND) Pack<T, V>::ld(w + (size_t)i * V, wv[c]);
+      P::ld(xr + (size_t)i * V, v[c]);
+      if constexpr (ADD) P::ld(mix + row * mix_stride + (size_t)i * V, m[c]);
+      if constexpr (!ROUND) P::ld(w + (size_t)i * V, wv[c]);
     }
   }
 #pragma unroll
@@ -106,7 +122,7 @@ __global__ void __launch_bounds__(ROUND ? 256 : 1024) rmsnorm_fp8_kernel(const T
       if constexpr (ADD) {
 #pragma unroll
         for (int j = 0; j < V; ++j) v[c][j] = Ty<T>::rnd(v[c][j] + m[c][j]);
-        Pack<T, V>::st(residual + row * cols + (size_t)i * V, v[c]);
+        P::st(residual + row * cols + (size_t)i * V, v[c]);
       }
 #pragma unroll
       for (int j = 0; j < V; ++j) ss += v[c][j] * v[c][j];
@@ -126,7 +142,7 @@ __global__ void __launch_bounds__(ROUND ? 256 : 1024) rmsnorm_fp8_kernel(const T
     for (int c = 0; c < NV; ++c) {
       const int i = (int)threadIdx.x + c * nt;
       if (i < n) {
-        Pack<T, V>::ld(w + (size_t)i * V, wv[0]);
+        P::ld(w + (size_t)i * V, wv[0]);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           v[c][j] = Ty<T>::rnd(v[c][j] * inv * (wv[0][j] + wofs));
@@ -149,7 +165,7 @@ __global__ void __launch_bounds__(ROUND ? 256 : 1024) rmsnorm_fp8_kernel(const T
       float y[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) y[j] = ROUND ? v[c][j] / scale : v[c][j] * f;
-      store_codes<V>(out + row * cols + (size_t)i * V, y);
+      store_codes<V, WIDE && V != 1>(out + row * cols + (size_t)i * V, y);
     }
   }
 }
@@ -265,12 +281,15 @@ cudaError_t launch(const T* x, size_t xs, const T* mix, size_t ms, const T* w, T
   auto al = [](const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; };
   const bool wide = cols % V == 0 && xs % V == 0 && al(x, 16) && al(w, 16) && al(out, V) && (!ADD || (ms % V == 0 && al(mix, 16) && al(res, 16)));
   if constexpr (ROUND) {  // the blocks and the summation order of the norm kernels whose bits it has to give (256 threads, f32 rows one element at a time)
-    if (sizeof(T) == 2 && wide && cols <= V * 4 * 256)
-      rmsnorm_fp8_kernel<T, V, 4, ADD, true><<<rows, 256, 0, s>>>(x, xs, mix, ms, w, res, out, scales, cols, eps, wofs, clip);
-    else if (cols <= 8 * 256)
-      rmsnorm_fp8_kernel<T, 1, 8, ADD, true><<<rows, 256, 0, s>>>(x, xs, mix, ms, w, res, out, scales, cols, eps, wofs, clip);
-    else
-      rmsnorm_fp8_long_kernel<T, ADD, true><<<rows, 256, 0, s>>>(x, xs, mix, ms, w, res, out, scales, cols, eps, wofs, clip);
+    if constexpr (sizeof(T) == 2) {
+      if (cols % V == 0 && cols <= V * 4 * 256) {  // eight elements a thread, off 16 bytes too
+        if (wide) rmsnorm_fp8_kernel<T, V, 4, ADD, true><<<rows, 256, 0, s>>>(x, xs, mix, ms, w, res, out, scales, cols, eps, wofs, clip);
+        else rmsnorm_fp8_kernel<T, V, 4, ADD, true, false><<<rows, 256, 0, s>>>(x, xs, mix, ms, w, res, out, scales, cols, eps, wofs, clip);
+        return cudaGetLastError();
+      }
+    }
+    if (cols <= 8 * 256) rmsnorm_fp8_kernel<T, 1, 8, ADD, true><<<rows, 256, 0, s>>>(x, xs, mix, ms, w, res, out, scales, cols, eps, wofs, clip);
+    else rmsnorm_fp8_long_kernel<T, ADD, true><<<rows, 256, 0, s>>>(x, xs, mix, ms, w, res, out, scales, cols, eps, wofs, clip);
   } else {
     auto threads = [](int items, int per) { return ((items + per - 1) / per + 31) / 32 * 32; };
     if (wide && cols <= V * 1024 && rows <= 1 << 30) {  // the row number may pass `rows` by the grid
