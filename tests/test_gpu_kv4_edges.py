@@ -228,3 +228,41 @@ def test_rounded_norm_has_the_bits_of_the_two_calls_off_16_bytes_too(G, dtype, r
         else:
             G.call("dcd_k_rmsnorm_fp8", xs, xs.stride(0), ws, q2, sc2, rows, cols, 1e-6, 1, 1.0, 1, dtype, None)
         assert torch.equal(sc, sc2) and torch.equal(q, q2)
+
+
+@pytest.mark.parametrize("add", [False, True])
+def test_rounded_norm_of_narrow_rows_is_not_slower_than_the_two_calls(G, add):
+    import torch
+    from decidra_b200 import _lib
+    lib, rows, cols = _lib.load(), 20000, 256
+    g = gen(8)
+    x, mix, w = normal(g, rows, cols), normal(g, rows, cols), normal(g, cols, by=0.1)
+    y, r, q, sc = torch.empty_like(x), torch.empty_like(x), torch.empty((rows, cols), dtype=torch.uint8, device="cuda"), torch.empty(rows, device="cuda")
+    px, pm, pw, py, pr, pq, ps = (C.c_void_p(a.data_ptr()) for a in (x, mix, w, y, r, q, sc))
+
+    def two():
+        if add:
+            assert lib.dcd_k_add_rmsnorm(px, pm, pw, pr, py, rows, cols, 1e-6, 1, None) == 0
+        else:
+            assert lib.dcd_k_rmsnorm(px, pw, py, rows, cols, 1e-6, 1, 1, None) == 0
+        assert lib.dcd_k_quant_fp8_rows(py, cols, pq, ps, rows, cols, 1.0, 1, None) == 0
+
+    def one():
+        if add:
+            assert lib.dcd_k_add_rmsnorm_fp8(px, cols, pm, cols, pw, pr, pq, ps, rows, cols, 1e-6, 1, 1.0, 1, 1, None) == 0
+        else:
+            assert lib.dcd_k_rmsnorm_fp8(px, cols, pw, pq, ps, rows, cols, 1e-6, 1, 1.0, 1, 1, None) == 0
+
+    took = []
+    for call in (two, one):
+        times = []
+        for _ in range(10):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(10):
+                call()
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        took.append(sorted(times)[5])
+    assert took[1] < took[0], took
