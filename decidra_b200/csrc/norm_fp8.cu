@@ -266,8 +266,6 @@ __global__ void __launch_bounds__(1024) rmsnorm_fp8_long_kernel(const T* x, size
   }
 }
 
-constexpr int ROWS_THREADS = 1344;  // resident threads of an SM at the 45 registers of rmsnorm_fp8_rows_kernel: one wave of its CTAs
-
 int sm_count() {
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) return 148;
@@ -297,7 +295,12 @@ cudaError_t launch(const T* x, size_t xs, const T* mix, size_t ms, const T* w, T
   } else {
     if (wide && cols <= V * 1024 && rows <= 1 << 30) {  // the row number may pass `rows` by the grid
       const int nt = threads(cols / V, 1);
-      const int grid = min(rows, sm_count() * (ROWS_THREADS / nt));
+      const int sms = sm_count();
+      int grid = rows, per_sm = 0;
+      if (rows > sms) {  // one wave; how many CTAs that is depends on the form's registers (a question of 0.4 us on the host)
+        CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, rmsnorm_fp8_rows_kernel<T, V, ADD>, nt, 0));
+        grid = min(rows, sms * max(1, per_sm));
+      }
       rmsnorm_fp8_rows_kernel<T, V, ADD><<<grid, nt, 0, s>>>(x, xs, mix, ms, w, res, out, scales, rows, cols, eps, wofs, clip);
     } else if (wide && cols <= V * 4 * 1024)
       rmsnorm_fp8_kernel<T, V, 4, ADD, false><<<rows, threads(cols / V, 4), 0, s>>>(x, xs, mix, ms, w, res, out, scales, cols, eps, wofs, clip);

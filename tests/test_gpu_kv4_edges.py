@@ -4,7 +4,7 @@ import ctypes as C
 
 import pytest
 
-from test_gpu_kv4 import Decode, Questions, attend, gen, normal, values
+from test_gpu_kv4 import Decode, Questions, attend, gen, norm_call, norm_check, normal, values
 
 pytestmark = pytest.mark.gpu
 
@@ -266,3 +266,13 @@ def test_rounded_norm_of_narrow_rows_is_not_slower_than_the_two_calls(G, add):
             times.append(a.elapsed_time(b))
         took.append(sorted(times)[5])
     assert took[1] < took[0], took
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("rows,cols", [(147, 5120), (149, 5120), (9500, 64), (20000, 256), (2000, 1024), (900, 4096)])
+def test_norm_of_many_rows(G, dtype, rows, cols):
+    """Fewer rows than a wave has CTAs, a few more, and many: every CTA takes its rows in turn."""
+    g = gen(rows)
+    x, mix, w = normal(g, rows, cols, dtype=dtype, by=3.0), normal(g, rows, cols, dtype=dtype), normal(g, cols, dtype=dtype, by=0.1)
+    norm_check(x, None, w, 1, 1.0, *norm_call(G, x, None, w, cols))
+    norm_check(x, mix, w, 1, 1.0, *norm_call(G, x, mix, w, cols))
