@@ -75,7 +75,8 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// sigmoid with the hardware exponential and reciprocal (2 ulp or so in f32; the product is rounded to bf16)
+// sigmoid with the hardware exponential and reciprocal (2 ulp or so in f32, 0 below 2^-126; the product is rounded to bf16). Split and whole
+// questions share it
 __device__ __forceinline__ float gate_of(float g) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(g * -1.4426950408889634f)));
@@ -860,8 +861,8 @@ __global__ void __launch_bounds__(128) kv4_attention_merge_kernel(const Params p
     float a = acc[i] * inv, b = acc[i + 1] * inv;
     if (gate) {
       const __nv_bfloat162 g2 = *reinterpret_cast<const __nv_bfloat162*>(gate + i);
-      a *= sigmoid_f(__low2float(g2));
-      b *= sigmoid_f(__high2float(g2));
+      a *= gate_of(__low2float(g2));
+      b *= gate_of(__high2float(g2));
     }
     *reinterpret_cast<__nv_bfloat162*>(dst + i) = __floats2bfloat162_rn(a, b);
   }

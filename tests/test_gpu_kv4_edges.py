@@ -276,3 +276,31 @@ def test_norm_of_many_rows(G, dtype, rows, cols):
     x, mix, w = normal(g, rows, cols, dtype=dtype, by=3.0), normal(g, rows, cols, dtype=dtype), normal(g, cols, dtype=dtype, by=0.1)
     norm_check(x, None, w, 1, 1.0, *norm_call(G, x, None, w, cols))
     norm_check(x, mix, w, 1, 1.0, *norm_call(G, x, mix, w, cols))
+
+
+# ---------------------------------------------------------------------------------------------
+# the gate
+# ---------------------------------------------------------------------------------------------
+def test_questions_have_one_gate_whether_their_keys_are_split_or_not(G):
+    """Scores of 0 over 4096 keys with V = 1 make 1 exactly, in one part or many: what is left is the gate's value, for every bf16 gate of
+    a magnitude below 128."""
+    import torch
+    n, S, heads, kv, hd = 16, 4080, 24, 4, 256
+    bits = torch.arange(0x4300, dtype=torch.int32, device="cuda")
+    gates = torch.cat((bits, bits + 0x8000)).to(torch.int16).view(torch.bfloat16)
+    outs = []
+    for others in (0, 160):
+        c = Questions([n] * (1 + others), S, heads, kv, hd, False, True)
+        c.q.zero_()
+        c.k.zero_()
+        c.v.fill_(1.0)
+        c.cache[2].fill_(0x22)
+        c.cache[3].fill_(0x38)
+        c.gate[:n, :, hd:] = gates.repeat(3)[:n * heads * hd].reshape(n, heads, hd)
+        c.launch(G)
+        torch.cuda.synchronize()
+        assert int(c.err.item()) == 0
+        outs.append(c.out[:n].clone())
+    want = torch.sigmoid(gates.double()).repeat(3)[:n * heads * hd].reshape(n, heads, hd)
+    assert ((outs[0].double() - want).abs() <= (2.0 ** -8 + 2.0 ** -21) * want + 2.0 ** -126).all()
+    assert torch.equal(outs[0], outs[1])
