@@ -1,10 +1,11 @@
 """The low-precision attention layer's kernels where they can go wrong unnoticed: work items of one key tile, values that are not finite
 in calls whose keys are split, loose bounds, offsets that fall, operands off their alignment, and every key counted once."""
 import ctypes as C
+import math
 
 import pytest
 
-from test_gpu_kv4 import Decode, Questions, attend, gen, norm_call, norm_check, normal, values
+from test_gpu_kv4 import Decode, Questions, attend, cu_of, gen, norm_call, norm_check, normal, values
 
 pytestmark = pytest.mark.gpu
 
@@ -304,3 +305,186 @@ def test_questions_have_one_gate_whether_their_keys_are_split_or_not(G):
     want = torch.sigmoid(gates.double()).repeat(3)[:n * heads * hd].reshape(n, heads, hd)
     assert ((outs[0].double() - want).abs() <= (2.0 ** -8 + 2.0 ** -21) * want + 2.0 ** -126).all()
     assert torch.equal(outs[0], outs[1])
+
+
+# ---------------------------------------------------------------------------------------------
+# every key once
+# ---------------------------------------------------------------------------------------------
+ONE = 0x38  # 1.0 in e4m3
+
+
+def dimension_of(j, hd, fine):
+    """The dimension in which key j has its only value: neighbouring keys in neighbouring ones, or sixteen keys in one."""
+    return (j if fine else j // 16) % hd
+
+
+def counting(codes, hd, j, fine):
+    """The rows of codes for keys j: 6 in one dimension, 0 elsewhere."""
+    import torch
+    d = dimension_of(j, hd, fine)
+    codes.zero_()
+    codes[torch.arange(len(j), device="cuda"), :, d // 2] = torch.where(d % 2 == 0, 7, 0x70).to(torch.uint8)[:, None].expand(-1, codes.shape[1])
+
+
+def counted(got, sees, hd, fine):
+    """With all scores 0 a token that sees n keys gives 6 / n for each one that has its value in a dimension: exact but for the division's and
+    the output's rounding. In the fine form a key that is missing, or there twice, is one of at most 128; in the other sixteen keys are."""
+    import torch
+    for i, n in enumerate(sees):
+        want = torch.bincount(dimension_of(torch.arange(n, device="cuda"), hd, fine), minlength=hd).double() * 6 / max(n, 1)
+        assert ((got[i].double() - want).abs() <= (2.0 ** -8 + 2.0 ** -21) * want).all(), (i, n)
+
+
+COUNTS = [(24, 4, 256), (16, 2, 128), (4, 1, 64), (15, 3, 256), (8, 8, 64)]
+
+
+@pytest.mark.parametrize("heads,kv,hd", COUNTS)
+@pytest.mark.parametrize("lens,L,fine", [([16384], 1, True), ([30000, 700, 1, 0, 33], 4, False), ([100 + 37 * i for i in range(40)], 1, True), ([12345, 64, 31, 5000], 2, True),
+                                         ([100000], 1, False)])
+def test_new_tokens_count_every_key_once(G, heads, kv, hd, lens, L, fine):
+    import torch
+    fine = fine and max(lens) <= 128 * hd
+    c = Decode(lens, L, heads, kv, hd)
+    c.q.zero_()
+    for s, n in zip(c.start, lens):
+        counting(c.cache[2][s:s + n], hd, torch.arange(n, device="cuda"), fine)
+        c.cache[3][s:s + n] = ONE
+    c.launch(G)
+    torch.cuda.synchronize()
+    assert int(c.err.item()) == 0
+    counted(c.out[:c.n], [max(0, n - L + 1 + i) for n in lens for i in range(L)], hd, fine)
+
+
+@pytest.mark.parametrize("heads,kv,hd", COUNTS)
+@pytest.mark.parametrize("lens,S,causal", [([16], 4096, False), ([16, 5], 16000, True), ([1], 1025, False), ([20] * 60, 2049, False), ([700, 900], 0, True), ([500, 127, 129, 1], 300, True),
+                                           ([1500], 0, False)])
+def test_questions_count_every_key_once(G, heads, kv, hd, lens, S, causal):
+    import torch
+    fine = S <= 100 * hd
+    c = Questions(lens, S, heads, kv, hd, causal, False)
+    c.q.zero_()
+    counting(c.cache[2][:S], hd, torch.arange(S, device="cuda"), fine)
+    c.cache[3][:S] = ONE
+    at, sees = 0, []
+    for n in lens:
+        d = dimension_of(torch.arange(S, S + n, device="cuda"), hd, fine)
+        own = torch.zeros(n, kv, hd, device="cuda", dtype=torch.bfloat16)
+        own[torch.arange(n, device="cuda"), :, d] = 6.0
+        c.v[at:at + n] = own.reshape(n, kv * hd)
+        sees += [S + (i + 1 if causal else n) for i in range(n)]
+        at += n
+    c.launch(G)
+    torch.cuda.synchronize()
+    assert int(c.err.item()) == 0
+    counted(c.out[:c.n], sees, hd, fine)
+
+
+@pytest.mark.parametrize("heads,kv,hd", [(24, 4, 256), (16, 2, 128), (4, 1, 64)])
+@pytest.mark.parametrize("lens,L", [([2000] * 64, 1), ([40000], 1), ([3000] * 20, 4), ([33] * 40, 2)])
+def test_new_tokens_find_one_key_wherever_it_is(G, heads, kv, hd, lens, L):
+    """A key whose score is hundreds above all others, at blocks' and parts' borders and in the last rows: its value comes back exactly."""
+    import torch
+    c = Decode(lens, L, heads, kv, hd)
+    c.q.fill_(1.0)
+    n, v = lens[0], values(*c.cache[2:])
+    spots = [0, 31, 32, n - L, n // 2, n - 33, n - 32] + [(2 * i + 1) * n // 120 for i in range(60)] + [32 * i % n for i in range(5, 400, 13)] + [32 * i % n + 31 for i in range(7, 400, 31)]
+    spots = [p for p in spots if 0 <= p <= n - L]
+    for first in range(0, len(spots), len(lens)) if len(lens) > 1 else range(0, len(spots), 6):
+        planted = [(spots + spots)[(first + b) % len(spots)] for b in range(len(lens))]
+        c.cache[0].zero_()
+        for s, p in zip(c.start, planted):
+            c.cache[0][s + p] = 0x77
+            c.cache[1][s:s + n] = ONE
+            c.cache[1][s + p] = 0x50  # 8: the key is 48 in every dimension
+        c.launch(G)
+        torch.cuda.synchronize()
+        assert int(c.err.item()) == 0
+        want = torch.stack([v[s + p] for s, p in zip(c.start, planted) for _ in range(L)]).repeat_interleave(heads // kv, 1)
+        assert torch.equal(c.out[:c.n].double(), want), planted
+
+
+@pytest.mark.parametrize("heads,kv,hd", [(24, 4, 256), (16, 2, 128), (4, 1, 64)])
+@pytest.mark.parametrize("lens,S", [([16], 4096), ([5, 9], 16001), ([20] * 64, 2048), ([300, 200], 100)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_questions_find_one_key_wherever_it_is(G, heads, kv, hd, lens, S, causal):
+    import torch
+    c = Questions(lens, S, heads, kv, hd, causal, False)
+    c.q.fill_(1.0)
+    vs = values(*c.cache[2:])[:S]
+    c.k.zero_()
+    for p in [0, 15, 16, 127, 128, 129, S - 1, S - 128, S // 2, S // 3] + [S * i // 13 // 128 * 128 + (i % 3 - 1) * 127 for i in range(1, 13)]:
+        p = min(max(p, 0), S - 1)
+        c.cache[0][:S].zero_()
+        c.cache[1][:S] = ONE
+        c.cache[0][p], c.cache[1][p] = 0x77, 0x50
+        c.launch(G)
+        torch.cuda.synchronize()
+        assert int(c.err.item()) == 0
+        assert torch.equal(c.out[:c.n].double(), vs[p].repeat_interleave(heads // kv, 0).expand(c.n, heads, hd)), p
+    # one of the question's own: its last key, which under causal only the last token sees
+    c.cache[0][:S].zero_()
+    ends = torch.tensor(cu_of(lens)[1:], device="cuda") - 1
+    c.k[ends] = 48.0
+    c.launch(G)
+    torch.cuda.synchronize()
+    for a, b in zip(cu_of(lens), cu_of(lens)[1:]):
+        rows = slice(b - 1, b) if causal else slice(a, b)
+        assert torch.equal(c.out[rows], c.v[b - 1].reshape(kv, hd).repeat_interleave(heads // kv, 0).expand(rows.stop - rows.start, heads, hd))
+
+
+def rounded_within(got, q, k, v, seen, p_step):
+    """A bound on each row's error as a whole. The output's rounding is at most 2^-8 of it; the weights' roundings, at most p_step of each, are
+    independent of one another and of the values, so that in the mean over the dimensions they add up as squares: p_step * sqrt(sum p^2 v^2).
+    Half as much again covers the mean's own scatter over 64 dimensions and more. A block of 32 keys of some thousand, left out or taken
+    twice, is more than twice that, where it is a small part of the bound on a single value."""
+    import torch
+    rep = q.shape[1] // k.shape[1]
+    k, v = (a.double().repeat_interleave(rep, 1) for a in (k, v))
+    s = torch.einsum("ihd,jhd->hij", q.double(), k) / math.sqrt(q.shape[2])
+    p = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
+    want = torch.einsum("hij,jhd->ihd", p, v)
+    noise = torch.einsum("hij,jhd->ihd", p.square(), v.square()).mean(-1).sqrt()
+    off = (got.double() - want).square().mean(-1).sqrt()
+    bound = 2.0 ** -8 * want.square().mean(-1).sqrt() + 1.5 * p_step * noise
+    assert (off <= bound).all(), float((off / bound).max())
+    # ... and the bound sees a block: the same rows without the last 32 keys that all of them see
+    m = int(seen.all(0).nonzero().max()) + 1
+    if m > 1000:
+        less = seen.clone()
+        less[:, m - 32:m] = False
+        p = torch.softmax(s.masked_fill(~less, -math.inf), -1)
+        short = (torch.einsum("hij,jhd->ihd", p, v) - want).square().mean(-1).sqrt()
+        assert (short > bound).double().mean() > 0.9
+
+
+@pytest.mark.parametrize("heads,kv,hd,lens,L", [(24, 4, 256, [16384], 1), (24, 4, 256, [5000, 1, 12345], 1), (16, 2, 128, [30000, 700], 4), (4, 1, 64, [9000] * 3, 2), (16, 1, 128, [4000, 100], 40)])
+def test_new_tokens_whole_rows(G, heads, kv, hd, lens, L):
+    import torch
+    c = Decode(lens, [min(L, n) for n in lens], heads, kv, hd)
+    c.q *= 0.4  # scores of about one: thousands of keys count
+    c.launch(G)
+    torch.cuda.synchronize()
+    k, v = values(*c.cache[:2]), values(*c.cache[2:])
+    at = 0
+    for s, n, m in zip(c.start, lens, c.L):
+        seen = torch.arange(n, device="cuda")[None] <= (n - m + torch.arange(m, device="cuda"))[:, None]
+        rounded_within(c.out[at:at + m], c.q[at:at + m].reshape(m, heads, hd), k[s:s + n], v[s:s + n], seen, 2.0 ** -11)
+        at += m
+
+
+@pytest.mark.parametrize("heads,kv,hd,lens,S,causal", [(24, 4, 256, [16], 4096, False), (24, 4, 256, [16, 5], 16384, True), (16, 2, 128, [1, 2], 9000, True), (4, 1, 64, [700, 900], 0, True),
+                                                       (24, 4, 256, [40] * 40, 2048, False)])
+def test_questions_whole_rows(G, heads, kv, hd, lens, S, causal):
+    import torch
+    c = Questions(lens, S, heads, kv, hd, causal, False)
+    c.q *= 0.4
+    c.launch(G)
+    torch.cuda.synchronize()
+    ks, vs = values(*c.cache[:2])[:S], values(*c.cache[2:])[:S]
+    for a, b in list(zip(cu_of(lens), cu_of(lens)[1:]))[:4]:
+        n = b - a
+        k, v = (torch.cat((x, y[a:b].double().reshape(n, kv, hd))) for x, y in ((ks, c.k), (vs, c.v)))
+        seen = torch.ones(n, S + n, dtype=torch.bool, device="cuda")
+        if causal:
+            seen[:, S:] = seen[:, S:].tril()
+        rounded_within(c.out[a:b], c.q[a:b], k, v, seen, 2.0 ** -8)
