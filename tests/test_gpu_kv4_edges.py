@@ -488,3 +488,42 @@ def test_questions_whole_rows(G, heads, kv, hd, lens, S, causal):
         if causal:
             seen[:, S:] = seen[:, S:].tril()
         rounded_within(c.out[a:b], c.q[a:b], k, v, seen, 2.0 ** -8)
+
+
+# ---------------------------------------------------------------------------------------------
+# sizes at the edge
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("heads,kv,hd", [(192, 1, 64), (131, 1, 64), (256, 2, 128), (129, 1, 256)])
+def test_more_query_heads_than_a_tile_has_rows(G, heads, kv, hd):
+    """Groups above 128 heads: cut into equal parts where they divide, a head at a time where they do not."""
+    for lens, S, causal in (([3, 40], 70, False), ([17], 0, True), ([5], 2000, True)):
+        c = Questions(lens, S, heads, kv, hd, causal, True)
+        c.launch(G)
+        c.check()
+    c = Decode([300, 5, 2000], [1, 2, 3], heads, kv, hd, gate=True)
+    c.launch(G)
+    c.check()
+
+
+def test_new_tokens_of_empty_stretches_at_the_ends_of_the_cache(G):
+    import torch
+    c = Decode([0, 40, 0, 0], [1, 2, 3, 1], 24, 4, 256, max_len=64)
+    c.t_start.copy_(torch.tensor([0, c.start[1], c.pool, c.pool]))
+    c.launch(G)
+    c.check()
+
+
+def test_calls_without_an_error_word(G):
+    import torch
+    for c in (Questions([5, 30], 3000, 24, 4, 256, False, True), Decode([2000, 3], 2, 24, 4, 256)):
+        keep = c.err
+        c.err = None
+        c.launch(G)
+        c.err = keep
+        c.check()
+    q = Questions([5, 30], 300, 24, 4, 256, False, True)
+    q.cu[1] = 99
+    q.err = None
+    q.launch(G)
+    torch.cuda.synchronize()
+    assert (q.out == -7.0).all()
