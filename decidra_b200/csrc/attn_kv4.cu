@@ -14,7 +14,9 @@
 //                  exponentials the other is in the barriers, TMEM loads and stores around its own, so neither unit waits for a
 //                  round trip, and no row is split between threads. Rescaling is lazy: O is rescaled only when a row's maximum has
 //                  grown by more than 2^8; the groups hand the maximum in use from tile to tile through shared memory.
-//   O += P V       P as the TMEM operand (over S[j]), V from shared memory, O in TMEM
+//   O += P V       P as the TMEM operand (over S[j]), V from shared memory, O in TMEM. The weights enter it as bf16, as they do in the
+//                  framework's bf16 attention (the operand has to be V's type): at most 2^-8 of each, independent of one another. Their sum is
+//                  taken in f32 before that. Against 64 bits the output's rms error is 0.0020 to 0.0023 of it, where rounding it alone leaves 0.0016
 // The tensor core runs S[0], S[1], then P.V[j], S[j + 2] in turn, so a tile's softmax has a whole tile's products to hide behind; up to
 // head_dim 128 TMEM holds a third S, and a group finds its next scores there when it has written its weights (head_dim 128: 980 -> 885 ns
 // a tile, 64: 965 -> 800). One warp issues both products: S[j + 2] overwrites P[j], and only one thread's products are sure to run in
@@ -31,7 +33,8 @@
 //
 // Few items over many keys leave SMs idle; the key tiles are then split into parts, items of their own, which a second kernel adds up.
 //
-// 64 questions of about 107 tokens over 2048 rows, 24 heads of 256, gated: 322 to 333 us, 1080 TFLOP/s of the 1648 that a library product reaches;
+// 64 questions of about 107 tokens over 2048 rows, 24 heads of 256, gated: 322 to 337 us (385 to 400 one after the other for 20 ms and more: the
+// power limit), 1050 to 1090 TFLOP/s of the 1648 that a library product reaches;
 // the tensor pipe is busy 56 % of the time, a tile takes 2400 to 2600 cycles for 2048 of products (S[j + 2] waits for P.V[j]), and a
 // quarter of an item is its start, its masked tile and its rows. Five causal prompts of 1051 to 1814 tokens, 16 heads of 128: 67 to 83 us,
 // bounded by the issue slots that the softmax and the issuing warp share.
@@ -945,8 +948,9 @@ cudaError_t run(const Kv4QuestionArgs& a, const Plan& pl, uint8_t* ws, cudaStrea
   if (items > (1 << 30)) return cudaErrorInvalidValue;
   const unsigned grid = (unsigned)max(min(items, (long long)sm_count()), (items + MAX_ITEMS - 1) / MAX_ITEMS);
   auto map = [](const TcTensorMap& m) -> const CUtensorMap& { return *reinterpret_cast<const CUtensorMap*>(&m); };
-  // started while the state is still being decoded: its setup and first Q lie under that (one question of 16 tokens over 4096 rows: 25.9 ->
-  // 24.0 us; with the merge started like this as well 29.3, and the same for the new tokens' merge gained nothing)
+  // started while the state is still being decoded: the setup of barriers and TMEM and the search for the items lie under that, every load waits
+  // for it (one question of 16 tokens over 4096 rows: 25.9 -> 24.0 us; with the merge started like this as well 29.3, and the same for
+  // the new tokens' merge gained nothing)
   if (a.n_state > 0) CUDA_TRY(launch_dependent(kv4_attention_kernel<HD>, grid, NUM_THREADS, Shape<HD>::SMEM, s, map(q), map(ksm), map(vsm), map(ko), map(vo), p));
   else kv4_attention_kernel<HD><<<grid, NUM_THREADS, Shape<HD>::SMEM, s>>>(map(q), map(ksm), map(vsm), map(ko), map(vo), p);
   CUDA_TRY(cudaGetLastError());

@@ -23,13 +23,14 @@
 // it, which keep an absolute error of 2^-25 of it), and the factor returns in the softmax scale. P is held as p * 2^10 in f16, so
 // that weights down to 2^-34 of the row's largest survive. Maxima, sums and O are f32.
 //
-// What bounds it: 64 sequences of 1024 to 16384 rows of 4 heads of 256 take 144 us, 4.4 TB/s (97 us at the copy rate). Of 1190 instructions
-// per 32 keys and head 512 convert and scale codes; 0.57 are issued a cycle and scheduler, the ALU pipe is 54 % busy, and 5 % of the stalls
-// wait for memory: the registers hold three warps a scheduler, and no more of them would fit. One token over 2048 rows takes 12.7 us, all
-// latency.
+// What bounds it: 64 sequences of 1024 to 16384 rows of 4 heads of 256 take 144 to 170 us, one machine and another, 4.4 to 3.7 TB/s (97 us at
+// the copy rate). Of 1190 instructions per 32 keys and head 512 convert and scale codes; 0.57 are issued a cycle and scheduler, the ALU
+// pipe is 54 % busy, and 5 % of the stalls wait for memory: the registers hold three warps a scheduler, and no more of them would fit.
+// One token over 2048 rows takes 12.2 to 15 us, all latency.
 //
 // Rows whose keys all went through one warp are finished there; otherwise each warp leaves its unnormalised O with maximum and sum in the
-// workspace, and a second kernel adds them up in their order. Keys beyond the stretch are zero-filled, masked keys get p = 0.
+// workspace, and a second kernel adds them up in their order. Keys beyond the stretch are zero-filled, masked keys get p = 0; a sum of 0 is a
+// token that sees no row, a sum of NaN stays NaN.
 #include "common.cuh"
 #include "kv4.h"
 
@@ -586,7 +587,8 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<HD, NT>::CTAS) kv4_decode_kern
 // out = sum_z O_z 2^(m_z - M) / sum_z l_z 2^(m_z - M). W warps per (token, head) take the parts in turn; their sums are added in
 // order. The row's sequence is found 32 offsets at a time, 32 parts' weights come at once, and the rows of four or eight parts are asked
 // for before the first is used: a chain of loads is what this kernel's time is made of (both kernels, one token over 8000 rows in 125
-// parts: 17 us; with a loop of one part after the other and never more than four warps 23.5; over 2048 rows 12.7 and 14.3).
+// parts: 14.7 us, over 2048 rows 12.4; when a row's parts lay further apart 17 and 12.7, and with a loop of one part after the other and never
+// more than four warps 23.5 and 14.3).
 template <int HD, int W>
 __global__ void __launch_bounds__(W > 4 ? W * 32 : 128) kv4_decode_merge_kernel(const Args p) {
   constexpr int WARPS_HERE = W > 4 ? W : 4, VEC = HD == 64 ? 2 : 4, NV = HD / 32 / VEC, U = W > 4 ? 8 : 4;  // a lane's values: VEC from lane * VEC on, NV times

@@ -8,7 +8,7 @@
 // Both kernels move each byte once and do a few operations a value: bound by HBM (write: 2 bytes a bf16 value in, 0.5625 out). One
 // thread handles one group of 16 of K and the same one of V, so that a warp's code words and scale bytes are contiguous and a thread has
 // both of its loads in flight; the 32 bytes of a bf16 group go in one 256-bit access (as two of 16 bytes each store would touch 32
-// sectors by half). 16384 rows of 4 heads of 256, there and back: 33.9 us for 172 MB (5.1 TB/s; 41.4 with 128-bit accesses and K and V in
+// sectors by half). 16384 rows of 4 heads of 256, there and back: 33.6 to 36.9 us for 172 MB (5.1 TB/s; 41.4 with 128-bit accesses and K and V in
 // different threads); 64 scattered rows 4.2 us, both launches.
 #include "common.cuh"
 #include "kv4.h"

@@ -561,9 +561,9 @@ DCD_API int dcd_k_add_rmsnorm(const void* x, const void* mix, const void* w, voi
  *   scales[row] = max(max|y| * clip, 1e-10) / 448; out [rows, cols] = e4m3_satfinite(y / scale).
  * x and mix are T with row strides in elements; residual may be x or mix itself where that one's stride is cols, and overlaps them in
  * no other way. round_t != 0 rounds y to T before it is quantised: the bits of dcd_k_rmsnorm / dcd_k_add_rmsnorm (zero_centered 1)
- * followed by dcd_k_quant_fp8_rows. round_t 0: y stays in f32 and is rounded once. Any cols; fastest where cols and the strides are
- * multiples of 8 (bf16) or 4 (f32) and the pointers 16-byte aligned. rows 0 does nothing
- * (its arrays may be NULL). */
+ * followed by dcd_k_quant_fp8_rows. round_t 0: y stays in f32, and the codes are those of (r * (w + zero_centered)) * ((1 / sqrt) / scale),
+ * within three f32 roundings of y / scale. Any cols; fastest where cols and the strides are multiples of 8 (bf16) or 4 (f32) and the
+ * pointers 16-byte aligned. rows 0 does nothing (its arrays may be NULL). */
 DCD_API int dcd_k_rmsnorm_fp8(const void* x, size_t x_stride, const void* w, void* out, float* scales, int rows, int cols, float eps, int zero_centered,
                               float clip, int round_t, int dtype, void* stream);
 DCD_API int dcd_k_add_rmsnorm_fp8(const void* x, size_t x_stride, const void* mix, size_t mix_stride, const void* w, void* residual, void* out,
@@ -684,13 +684,15 @@ DCD_API int dcd_k_kv4_read(const void* k_codes, const void* k_scales, const void
                            void* k, void* v, int rows, int kv, int hd, int dtype, int* err, void* stream);
 /* dcd_k_attention_tc over a 4-bit state: every packed question attends to the n_state rows of the cache and to its own bf16 keys (all
  * of them, or with causal != 0 those up to itself), out = softmax(q k / sqrt(hd)) v, times sigmoid(gate) where gate_qg (laid out as
- * there) is given. n_state 0 with causal 1 is causal attention over packed prompts; the cache pointers may then be NULL. bf16; any
- * heads that kv divides; hd 64, 128 or 256; q [T, heads, hd], k_own and v_own [T, kv, hd] with row strides in elements, multiples of 8,
- * 16-byte aligned, qg_stride at most 2^24; out [T, heads, hd]. cu_seqlens [B + 1] rises from 0 to at most T; a sequence whose offsets
- * fall or leave [0, T] sets *err and is left out, and rows of out that no sequence has, those behind the last one too, are left as they
- * were. A NaN or an infinity in a question's values may reach all of that question's tokens, later ones' under causal too (its weight
- * there is 0, and 0 times it is NaN), and nothing outside the question. workspace: dcd_k_attention_kv4_workspace bytes (0: none is
- * needed), 16-byte aligned, not shared by calls that may overlap. */
+ * there) is given; the weights enter the second product as bf16 (in the form for new tokens as f16), and output times sigmoid is rounded
+ * once, where dcd_k_attention_tc rounds either first. n_state 0 with causal 1 is causal attention over packed prompts; the cache
+ * pointers may then be NULL. bf16; any heads that kv divides; hd 64, 128 or 256; q [T, heads, hd], k_own and v_own [T, kv, hd] with row
+ * strides in elements, multiples of 8, 16-byte aligned, qg_stride at most 2^24; out [T, heads, hd]. cu_seqlens [B + 1] rises from 0 to
+ * at most T; a sequence whose offsets fall or leave [0, T] sets *err (which may be NULL) and is left out, and rows of out that no
+ * sequence has, those behind the last one too, are left as they were. A row with a score of NaN is NaN. A NaN or an infinity in a
+ * question's values may reach all of that question's tokens, later ones' under causal too (its weight there is 0, and 0 times it is
+ * NaN), and nothing outside the question. workspace: dcd_k_attention_kv4_workspace bytes for the call's sizes (0: none is needed; a
+ * smaller batch may need more, where its keys are split), 16-byte aligned, not shared by calls that may overlap. */
 DCD_API size_t dcd_k_attention_kv4_workspace(int B, int T, int n_state, int heads, int kv, int hd);
 DCD_API int dcd_k_attention_kv4(const void* q, size_t q_stride, const void* k_own, size_t k_stride, const void* v_own, size_t v_stride, const void* k_codes,
                                 const void* k_scales, const void* v_codes, const void* v_scales, int n_state, const void* gate_qg, size_t qg_stride,
@@ -699,9 +701,10 @@ DCD_API int dcd_k_attention_kv4(const void* q, size_t q_stride, const void* k_ow
 /* The form for new tokens: sequence b's rows in the cache are [seg_start[b], seg_start[b] + seg_len[b]), its packed tokens
  * [cu_seqlens[b], cu_seqlens[b + 1]) are the newest ones, already written there: the last token sees every row of the stretch, each
  * one before it a row less. Stretches may be shared or overlap. A token that sees no row (more tokens than rows) gives 0. A stretch
- * that leaves the cache or is longer than max_len sets *err, and its tokens give 0. max_len is at most 2^30; a bound far above
- * the lengths costs neither time nor memory (the workspace has a fixed part of up to 40 MB and, where kv is not a multiple of 4, one that
- * grows with T * heads). Meant for one to a few tokens a sequence; every other operand as above. */
+ * that leaves the cache or is longer than max_len sets *err, and its tokens give 0. max_len is at most 2^30; a bound far above the
+ * lengths costs neither time nor memory: the workspace has a part of at most 40 MB and, where kv is not a multiple of 4, one that grows
+ * with T * heads, and what is enough for the largest B, T and max_len is enough for smaller ones. Meant for one to a few tokens a
+ * sequence; every other operand as above. */
 DCD_API size_t dcd_k_attention_kv4_decode_workspace(int B, int T, int max_len, int heads, int kv, int hd);
 DCD_API int dcd_k_attention_kv4_decode(const void* q, size_t q_stride, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
                                        size_t cache_rows, const int64_t* seg_start, const int32_t* seg_len, int max_len, const void* gate_qg,
