@@ -115,6 +115,7 @@ struct Args {
   float* ws_o;     // [places][hd] unnormalised O of a part of a row
   float2* ws_ml;   // [places] (maximum in log2 units, sum)
   uint2* ws_n;     // [T * heads] the row's parts and the place of its first: they lie behind each other
+  int* ws_falls;   // some sequence's offsets fall or leave the batch
 };
 
 // The first place of a row of a pair that is split between CTAs from `first_cta` on. A warp's row has a place for every even number of a CTA
@@ -124,6 +125,7 @@ struct Args {
 __device__ __forceinline__ uint32_t split_place(int row, int first_cta, int step) { return ((uint32_t)row * gridDim.x + first_cta) * (2 * step); }
 
 struct Sequence {
+  bool sound;  // its offsets
   int off, L, len;
   size_t start;
 };
@@ -132,9 +134,9 @@ __device__ __forceinline__ Sequence sequence(const Kv4DecodeArgs& a, int b, bool
   Sequence s;
   s.off = a.cu[b];
   const int stop = a.cu[b + 1];
-  const bool sound = s.off >= 0 && stop >= s.off && stop <= a.T;  // compared before they are subtracted: the difference of bad ones may overflow
-  s.L = sound ? stop - s.off : 0;
-  if (!sound && report) set_err(a.err, DERR_OFFSETS);
+  s.sound = s.off >= 0 && stop >= s.off && stop <= a.T;  // compared before they are subtracted: the difference of bad ones may overflow
+  s.L = s.sound ? stop - s.off : 0;
+  if (!s.sound && report) set_err(a.err, DERR_OFFSETS);
   const int64_t st = a.seg_start[b];
   s.len = a.seg_len[b];
   s.start = (size_t)st;
@@ -210,9 +212,15 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<HD, NT>::CTAS) kv4_decode_kern
   {
     const int per = (a.B + WARPS * 32 - 1) / (WARPS * 32), b0 = min((int)threadIdx.x * per, a.B), b1 = min(b0 + per, a.B);
     long long mine = 0;
+    int falls = 0;
     for (int i = b0; i < b1; ++i) {
       const Sequence s = sequence(a, i, blockIdx.x == 0);
+      falls |= !s.sound;
       mine += (long long)n_groups * rounds_of<ROWS>(s, G) * blocks_of(s);
+    }
+    if (blockIdx.x == 0) {
+      falls = __syncthreads_or(falls);
+      if (threadIdx.x == 0) *p.ws_falls = falls;
     }
     long long before = mine, total = 0;
 #pragma unroll
@@ -616,8 +624,9 @@ __global__ void __launch_bounds__(W > 4 ? W * 32 : 128) kv4_decode_merge_kernel(
       return off >= 0 && off <= t && t < end && end <= a.T;
     };
     bool mine = has(lo);
-    // not there: a row behind the last sequence, or offsets that fall, among which a sound sequence may have been missed
-    for (int i = lane; !mine && i - lane < a.B; i += 32) mine = __any_sync(0xffffffffu, i < a.B && has(i));
+    // not there: a row behind the last sequence, or, where some offsets fall, one of a sound sequence that was missed
+    if (!mine && *p.ws_falls)
+      for (int i = lane; !mine && i - lane < a.B; i += 32) mine = __any_sync(0xffffffffu, i < a.B && has(i));
     if (mine) {
       const uint2 n = p.ws_n[at];
       nz = (int)n.x;
@@ -750,7 +759,7 @@ cudaError_t run(const Args& p, const Plan& plan, cudaStream_t s) {
 
 size_t kv4_decode_workspace(int B, int T, int max_len, int heads, int kv, int hd) {
   const kvd::Plan p = kvd::plan_of(B, T, max_len, heads, kv, hd);
-  return p.places * ((size_t)hd * sizeof(float) + sizeof(float2)) + (size_t)T * heads * sizeof(uint2);
+  return p.places * ((size_t)hd * sizeof(float) + sizeof(float2)) + (size_t)T * heads * sizeof(uint2) + sizeof(int);
 }
 
 cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, void* workspace, cudaStream_t s) {
@@ -764,6 +773,7 @@ cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, void* workspace, cudaStrea
   p.ws_o = (float*)workspace;
   p.ws_ml = (float2*)(p.ws_o + plan.places * a.hd);
   p.ws_n = (uint2*)(p.ws_ml + plan.places);
+  p.ws_falls = (int*)(p.ws_n + (size_t)a.T * a.heads);
   if (a.hd == 256) return plan.nt == 1 ? kvd::run<256, 1>(p, plan, s) : kvd::run<256, 2>(p, plan, s);
   if (a.hd == 128) return plan.nt == 1 ? kvd::run<128, 1>(p, plan, s) : plan.nt == 2 ? kvd::run<128, 2>(p, plan, s) : kvd::run<128, 4>(p, plan, s);
   return plan.nt == 1 ? kvd::run<64, 1>(p, plan, s) : plan.nt == 2 ? kvd::run<64, 2>(p, plan, s) : kvd::run<64, 4>(p, plan, s);

@@ -191,6 +191,25 @@ def test_new_tokens_of_a_sound_sequence_behind_offsets_that_fall(G, cu, heads, k
     assert (c.out[[t for t in range(12) if t not in taken]] == -7.0).all()
 
 
+def test_new_tokens_rows_behind_the_last_sequence_cost_little(G):
+    """A call at a server's capacity: 4096 sequences, and room for twice as many tokens as they have."""
+    import torch
+    took = []
+    for behind in (0, 4096):
+        c = Decode([5] * 4096, 1, 24, 4, 256, behind=behind)
+        times = []
+        for _ in range(6):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            c.launch(G)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        took.append(sorted(times)[2])
+        assert (c.out[c.n:] == -7.0).all()
+    assert took[1] < 1.5 * took[0], took
+
+
 # ---------------------------------------------------------------------------------------------
 # the norm's rounded form
 # ---------------------------------------------------------------------------------------------
