@@ -705,15 +705,14 @@ kv4_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         gv[ps] = ld_global_if(gate0 + gate_at[ps] + c, out_at[ps] != ~0u);
     };
     if (gate0) load_gates(0);
-    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar_m + 8 * last, (uint32_t)(last_j >> 1) & 1, abort_flag));
+    // The maximum in use at the end, from the group of the last tile. The other group may still be reading this group's sums of the item before;
+    // with two tiles or more it has published a maximum of this item since, and that was waited for. The owner of an item's only tile has
+    // the maximum itself and waits for the item before in its place.
+    const bool only = n_tiles == 1 && h == last && live > 0;
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(only ? bar_o_free : bar_m + 8 * last, (uint32_t)(only ? live - 1 : last_j >> 1) & 1, abort_flag));
     float end_m = -INFINITY;
     if (ok) {
       end_m = m_used[last * 128 + r];
-      // The other group may still be reading this group's sums of the item before. With two tiles or more it has published a maximum of this
-      // item since, and that was waited for; the owner of an item's only tile has waited for nothing of the other group.
-      if (n_tiles == 1 && live > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar_o_free, (uint32_t)(live - 1) & 1, abort_flag));
-    }
-    if (ok) {
       // a group that has seen no score: m = -inf and l = 0, or NaN where all of its scores were, which the sum has to show
       l_part[h * 128 + r] = m == -INFINITY ? l : l * ex2(m - end_m);
       mbar_arrive(bar_l);
