@@ -692,7 +692,8 @@ DCD_API int dcd_k_kv4_read(const void* k_codes, const void* k_scales, const void
  * sequence has, those behind the last one too, are left as they were. A row with a score of NaN is NaN. A NaN or an infinity in a
  * question's values may reach all of that question's tokens, later ones' under causal too (its weight there is 0, and 0 times it is
  * NaN), and nothing outside the question. workspace: dcd_k_attention_kv4_workspace bytes for the call's sizes (0: none is needed; a
- * smaller batch may need more, where its keys are split), 16-byte aligned, not shared by calls that may overlap. */
+ * smaller batch may need more, where its keys are split), 16-byte aligned, not shared by calls that may overlap. Keys are split where B
+ * and T leave SMs idle, so that a T far above the batch's tokens keeps them whole and a long state's few tiles slow. */
 DCD_API size_t dcd_k_attention_kv4_workspace(int B, int T, int n_state, int heads, int kv, int hd);
 DCD_API int dcd_k_attention_kv4(const void* q, size_t q_stride, const void* k_own, size_t k_stride, const void* v_own, size_t v_stride, const void* k_codes,
                                 const void* k_scales, const void* v_codes, const void* v_scales, int n_state, const void* gate_qg, size_t qg_stride,
